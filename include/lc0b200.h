@@ -266,6 +266,48 @@ LC0B200_API int lc0b200_linear_int8_static(void* out_bf16, const void* a_bf16, c
                                const float* col_scale, const void* bias_bf16, long long m, int n, int k,
                                int activation, void* stream);
 
+/* ---- 8-bit floating point (e4m3) ----------------------------------------------------------
+ *
+ * No reference counterpart (the reference has no 8-bit path).  Codes are e4m3 (finite form: largest value 448, one NaN).
+ * The block rule, for the values x of one block of 128 (1 x 128 along a row) or 128 x 128 (weights):
+ *   amax = max |x| (a NaN stays one);  scale = amax / 448, or 1 where amax < 2^-117 (a block of zeros);
+ *   code = e4m3(x * (448 / amax)), factor 1 where amax < 2^-117; one IEEE division, fp32 product, round half to even,
+ *   saturated.  A block with an infinity or a NaN gets a non-finite scale and reads back as NaN throughout.
+ * The last block of a row (and the last rows of a matrix) may be short.  Scales of activations are block-major like the
+ * row statistics of lc0b200_gemm: scale[block * ld_scale + row], ld_scale >= rows; scales of weights are
+ * scale[(row / 128) * ld_scale + column / 128].  All ld* are row pitches in elements.  Outputs may not overlap inputs
+ * except where said.  Bytes between a row's width and its pitch are neither read nor written. */
+
+/* bf16 rows to codes; block_rows is 1 (activations) or 128 (weights, at load time).  Any alignment; 16-byte aligned
+ * input rows and 8-byte aligned output rows are the fast form. */
+LC0B200_API int lc0b200_quantize_fp8(void* out_e4m3, float* scale_f32, const void* in_bf16, long long row_count, int width,
+                                     int block_rows, long long ld_in, long long ld_out, long long ld_scale, void* stream);
+/* v = in + skip (skip may be NULL: v = in); residual_out = bf16(v) (may be NULL; needs skip);
+ * y = v / sqrt(mean(v^2) + epsilon) * gamma, fp32; out = bf16(y) and / or q_out, q_scale = block rule on y (each pair may
+ * be NULL, not both).  Every output is rounded once from its fp32 value.  out and residual_out may be in or skip
+ * themselves (same pointer and pitch).  A pitch belongs to its pointer and is ignored where that is NULL.
+ * A row whose mean square overflows fp32 (values above about 1e19) gives zeros. */
+LC0B200_API int lc0b200_rms_norm(void* out_bf16, void* residual_out_bf16, void* q_out_e4m3, float* q_scale_f32,
+                                 const void* in_bf16, const void* skip_bf16, const void* gamma_bf16, long long row_count,
+                                 int width, float epsilon, long long ld_in, long long ld_skip, long long ld_out,
+                                 long long ld_residual, long long ld_q, long long ld_scale, void* stream);
+/* out[m,n] = act(bias[n] + sum over 128-blocks b of k: a_scale[b,m] * w_scale[n / 128, b] * sum_{k in b} a[m,k] * w[n,k]),
+ * codes [m,k] and [n,k] row-major, fp32 sums, bias bf16 or NULL, out bf16 or f32 (out_kind).  The two scales of a block are
+ * multiplied in fp32 first, so their product has to be a finite fp32 number.  A NaN stays in its row of a and its
+ * column of w.  Bases and pitches of a and w that are multiples of 16 bytes run on the tensor cores, others on the CUDA
+ * cores (correct, slow).  The order of summation depends on the shape alone: the same call gives the same bits. */
+LC0B200_API int lc0b200_gemm_fp8(void* out, const void* a_e4m3, const float* a_scale, const void* w_nk_e4m3,
+                                 const float* w_scale, const void* bias_bf16, long long m, int n, int k, long long lda,
+                                 long long ld_a_scale, long long ldw, long long ld_w_scale, long long ldc, int out_kind,
+                                 int activation, void* stream);
+/* One e4m3 dense layer on bf16 activations: lc0b200_quantize_fp8 (1 x 128 blocks) into caller-provided scratch, then
+ * lc0b200_gemm_fp8.  scratch_q holds m * (k rounded up to 16) bytes, scratch_scale m * ceil(k / 128) floats; both 16-byte
+ * aligned, reusable as soon as the call's kernels have run (calls that may overlap need scratch of their own). */
+LC0B200_API int lc0b200_linear_fp8(void* out, const void* a_bf16, const void* w_nk_e4m3, const float* w_scale,
+                                   const void* bias_bf16, void* scratch_q, float* scratch_scale, long long m, int n, int k,
+                                   long long lda, long long ldw, long long ld_w_scale, long long ldc, int out_kind,
+                                   int activation, void* stream);
+
 /* ---- heads -------------------------------------------------------------------------------- */
 
 /* K/promotion_logits.py:67-145 (argument order records,keys,weights as the reference ABI):

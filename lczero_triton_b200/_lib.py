@@ -67,6 +67,10 @@ SIGNATURES: dict[str, tuple] = {
     "lc0b200_normalize_quantize_rows": (_P, _P, _P, _P, _I, _P, _P, _L, _I, _F, _P),
     "lc0b200_linear_int8": (_P, _P, _P, _P, _P, _P, _P, _L, _I, _I, _I, _P),
     "lc0b200_linear_int8_static": (_P, _P, _P, _P, _P, _L, _I, _I, _I, _P),
+    "lc0b200_quantize_fp8": (_P, _P, _P, _L, _I, _I, _L, _L, _L, _P),
+    "lc0b200_rms_norm": (_P, _P, _P, _P, _P, _P, _P, _L, _I, _F, _L, _L, _L, _L, _L, _L, _P),
+    "lc0b200_gemm_fp8": (_P, _P, _P, _P, _P, _P, _L, _I, _I, _L, _L, _L, _L, _L, _I, _I, _P),
+    "lc0b200_linear_fp8": (_P, _P, _P, _P, _P, _P, _P, _L, _I, _I, _L, _L, _L, _L, _I, _I, _P),
     "lc0b200_promotion_logits": (_P, _P, _P, _I, _I, _P),
     "lc0b200_embed_position_input": (_P, _P, _P, _I, _P),
     "lc0b200_embed_concat": (_P, _P, _P, _P, _I, _I, _P),

@@ -7,6 +7,7 @@
 
 #include "common.cuh"
 #include "gemm.h"
+#include "gemm_fp8.h"
 #include "kernels.h"
 
 namespace lc0b200 {
@@ -76,6 +77,9 @@ using namespace lc0b200;
   } while (0)
 
 static inline cudaStream_t S(void* stream) { return reinterpret_cast<cudaStream_t>(stream); }
+
+// Widths and inner lengths of the e4m3 operators: column indices rounded up to whole blocks stay within an int.
+constexpr int kMaxFp8Width = 1 << 30;
 
 static bool valid_activation(int a) { return a >= LC0B200_ACT_NONE && a <= LC0B200_ACT_SWISH; }
 
@@ -348,6 +352,81 @@ LC0B200_API int lc0b200_linear_int8(void* out, const void* a, const void* w_nk, 
   if (!valid_activation(activation)) return LC0B200_ERR_UNSUPPORTED;
   if (m == 0) return LC0B200_OK;
   return linear_int8(out, a, w_nk, col_scale, bias, scratch_q, scratch_scale, m, n, k, activation, S(stream));
+}
+
+LC0B200_API int lc0b200_quantize_fp8(void* out, float* scale, const void* in, long long row_count, int width, int block_rows,
+                                     long long ld_in, long long ld_out, long long ld_scale, void* stream) {
+  REQUIRE_PTR(out); REQUIRE_PTR(scale); REQUIRE_PTR(in);
+  REQUIRE_SHAPE(row_count >= 0 && row_count <= 0x7FFFFFFFLL && width > 0 && width <= kMaxFp8Width);
+  if (block_rows != 1 && block_rows != 128) return LC0B200_ERR_UNSUPPORTED;
+  REQUIRE_SHAPE(ld_in >= width && ld_out >= width);
+  REQUIRE_SHAPE(ld_scale >= (block_rows == 1 ? row_count : ceil_div_ll(width, 128)));
+  REQUIRE_ALIGNED(in, 2); REQUIRE_ALIGNED(scale, 4);
+  if (row_count == 0) return LC0B200_OK;
+  return quantize_fp8(out, scale, in, row_count, width, block_rows, ld_in, ld_out, ld_scale, S(stream));
+}
+
+LC0B200_API int lc0b200_rms_norm(void* out, void* residual_out, void* q_out, float* q_scale, const void* in, const void* skip,
+                                 const void* gamma, long long row_count, int width, float epsilon, long long ld_in,
+                                 long long ld_skip, long long ld_out, long long ld_residual, long long ld_q,
+                                 long long ld_scale, void* stream) {
+  REQUIRE_PTR(in); REQUIRE_PTR(gamma);
+  if (out == nullptr && q_out == nullptr) return LC0B200_ERR_NULL_POINTER;
+  if ((q_out == nullptr) != (q_scale == nullptr)) return LC0B200_ERR_NULL_POINTER;
+  if (residual_out != nullptr) REQUIRE_PTR(skip);  // without a skip operand the residual is the input itself
+  REQUIRE_SHAPE(row_count >= 0 && row_count <= 0x7FFFFFFFLL && width > 0 && width <= kMaxFp8Width && epsilon >= 0.0f);
+  REQUIRE_SHAPE(ld_in >= width);
+  REQUIRE_ALIGNED(in, 2); REQUIRE_ALIGNED(gamma, 2);
+  if (skip != nullptr) { REQUIRE_SHAPE(ld_skip >= width); REQUIRE_ALIGNED(skip, 2); }
+  if (out != nullptr) { REQUIRE_SHAPE(ld_out >= width); REQUIRE_ALIGNED(out, 2); }
+  if (residual_out != nullptr) { REQUIRE_SHAPE(ld_residual >= width); REQUIRE_ALIGNED(residual_out, 2); }
+  if (q_out != nullptr) { REQUIRE_SHAPE(ld_q >= width && ld_scale >= row_count); REQUIRE_ALIGNED(q_scale, 4); }
+  if (row_count == 0) return LC0B200_OK;
+  return rms_norm(out, residual_out, q_out, q_scale, in, skip, gamma, row_count, width, epsilon, ld_in, ld_skip, ld_out,
+                  ld_residual, ld_q, ld_scale, S(stream));
+}
+
+static int check_gemm_fp8(const GemmFp8& g) {
+  REQUIRE_PTR(g.out); REQUIRE_PTR(g.a); REQUIRE_PTR(g.a_scale); REQUIRE_PTR(g.w); REQUIRE_PTR(g.w_scale);
+  REQUIRE_SHAPE(g.m >= 0 && g.m <= 0x7FFFFF00LL && g.n > 0 && g.n <= kMaxFp8Width && g.k > 0 && g.k <= kMaxFp8Width);
+  REQUIRE_SHAPE(g.lda >= g.k && g.ldw >= g.k && g.ldc >= g.n);
+  REQUIRE_SHAPE(g.ld_a_scale >= g.m && g.ld_w_scale >= ceil_div_ll(g.k, 128));
+  if (g.out_kind != LC0B200_OUT_BF16 && g.out_kind != LC0B200_OUT_F32) return LC0B200_ERR_UNSUPPORTED;
+  if (!valid_activation(g.activation)) return LC0B200_ERR_UNSUPPORTED;
+  REQUIRE_ALIGNED(g.a_scale, 4); REQUIRE_ALIGNED(g.w_scale, 4);
+  REQUIRE_ALIGNED(g.out, g.out_kind == LC0B200_OUT_BF16 ? 2 : 4);
+  if (g.bias != nullptr) REQUIRE_ALIGNED(g.bias, 2);
+  return LC0B200_OK;
+}
+
+LC0B200_API int lc0b200_gemm_fp8(void* out, const void* a, const float* a_scale, const void* w_nk, const float* w_scale,
+                                 const void* bias, long long m, int n, int k, long long lda, long long ld_a_scale,
+                                 long long ldw, long long ld_w_scale, long long ldc, int out_kind, int activation,
+                                 void* stream) {
+  const GemmFp8 g = {out, reinterpret_cast<const uint8_t*>(a), a_scale, reinterpret_cast<const uint8_t*>(w_nk), w_scale,
+                     reinterpret_cast<const bf16*>(bias), m, n, k, lda, ld_a_scale, ldw, ld_w_scale, ldc, out_kind, activation};
+  const int st = check_gemm_fp8(g);
+  if (st != LC0B200_OK) return st;
+  if (m == 0) return LC0B200_OK;
+  return gemm_fp8(g, S(stream));
+}
+
+LC0B200_API int lc0b200_linear_fp8(void* out, const void* a, const void* w_nk, const float* w_scale, const void* bias,
+                                   void* scratch_q, float* scratch_scale, long long m, int n, int k, long long lda,
+                                   long long ldw, long long ld_w_scale, long long ldc, int out_kind, int activation,
+                                   void* stream) {
+  REQUIRE_PTR(a); REQUIRE_PTR(scratch_q); REQUIRE_PTR(scratch_scale);
+  REQUIRE_SHAPE(k > 0 && k <= kMaxFp8Width && lda >= k);
+  REQUIRE_ALIGNED(a, 2); REQUIRE_ALIGNED(scratch_q, 16); REQUIRE_ALIGNED(scratch_scale, 16);
+  const long long pitch = ceil_div_ll(k, 16) * 16;  // TMA wants rows at multiples of 16 bytes
+  const GemmFp8 g = {out, reinterpret_cast<const uint8_t*>(scratch_q), scratch_scale, reinterpret_cast<const uint8_t*>(w_nk),
+                     w_scale, reinterpret_cast<const bf16*>(bias), m, n, k, pitch, m, ldw, ld_w_scale, ldc, out_kind, activation};
+  int st = check_gemm_fp8(g);
+  if (st != LC0B200_OK) return st;
+  if (m == 0) return LC0B200_OK;
+  st = quantize_fp8(scratch_q, scratch_scale, a, m, k, 1, lda, pitch, m, S(stream));
+  if (st != LC0B200_OK) return st;
+  return gemm_fp8(g, S(stream));
 }
 
 LC0B200_API int lc0b200_promotion_logits(void* records, const void* keys, const void* w, int batch_size, int width,

@@ -1,0 +1,46 @@
+// The e4m3 block rule shared by the kernels that produce 8-bit floating rows.
+//
+// Block of 128 values (1 x 128 for activations, 128 x 128 for weights):
+//   amax  = max |x|                          a NaN stays a NaN, an infinity stays one
+//   scale = amax / 448                       1 where amax < 2^-117: such a block counts as zeros
+//   code  = e4m3(x * (448 / amax))           IEEE division once per block, round half to even, saturated to +-448
+// 2^-117 is where 448 / amax still is a finite float (it overflows below 2^-119.2).  Non-finite blocks cannot hide:
+// amax = inf gives scale = inf and codes 0 and NaN, amax = NaN gives scale = NaN, so every value of such a block
+// reads back as NaN.
+#pragma once
+
+#include <cuda_fp8.h>
+#include <stdint.h>
+
+#include "common.cuh"
+
+namespace lc0b200 {
+
+constexpr int kFp8Block = 128;
+constexpr float kFp8Max = 448.0f;
+constexpr uint32_t kFp8TinyBits = 0x05000000u;  // 2^-117 as float bits
+
+// |x| as bits: unsigned order is the order of magnitudes with every NaN above infinity, so an integer maximum keeps NaN.
+__device__ __forceinline__ uint32_t magnitude_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
+
+__device__ __forceinline__ void fp8_block_scale(uint32_t amax_bits, float& scale, float& inverse) {
+  const float amax = __uint_as_float(amax_bits);
+  const bool zeros = amax_bits < kFp8TinyBits;
+  scale = zeros ? 1.0f : __fdiv_rn(amax, kFp8Max);
+  inverse = zeros ? 1.0f : __fdiv_rn(kFp8Max, amax);
+}
+
+__device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return lo | (hi << 16);
+}
+
+__device__ __forceinline__ uint8_t fp8_one(float a) { return __nv_cvt_float_to_fp8(a, __NV_SATFINITE, __NV_E4M3); }
+
+__device__ __forceinline__ float fp8_value(uint8_t code) {
+  const __half_raw h = __nv_cvt_fp8_to_halfraw(code, __NV_E4M3);
+  return __half2float(__half(h));
+}
+
+}  // namespace lc0b200

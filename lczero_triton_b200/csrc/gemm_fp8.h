@@ -1,0 +1,29 @@
+// Internal: the back ends behind lc0b200_gemm_fp8 / lc0b200_linear_fp8 (validated arguments only).
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "common.cuh"
+
+namespace lc0b200 {
+
+struct GemmFp8 {
+  void* out;
+  const uint8_t* a;
+  const float* a_scale;
+  const uint8_t* w;
+  const float* w_scale;
+  const bf16* bias;
+  long long m;
+  int n, k;
+  long long lda, ld_a_scale, ldw, ld_w_scale, ldc;
+  int out_kind, activation;
+};
+
+// Chooses the kernel by what the operands allow.
+int gemm_fp8(const GemmFp8& g, cudaStream_t stream);
+// CUDA-core kernel: any pitch and alignment.
+int gemm_fp8_simt(const GemmFp8& g, cudaStream_t stream);
+
+}  // namespace lc0b200

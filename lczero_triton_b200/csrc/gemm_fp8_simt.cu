@@ -1,0 +1,79 @@
+// CUDA-core form of the block-scaled e4m3 product, for operands TMA cannot address (a base or a row pitch that is not a
+// multiple of 16 bytes) and as an independent cross-check of the tensor-core kernels.  64 x 64 output tile per CTA,
+// 4 x 4 per thread; codes are scaled to f32 as they enter shared memory.
+#include <cuda_runtime.h>
+
+#include "common.cuh"
+#include "fp8.cuh"
+#include "gemm_fp8.h"
+
+namespace lc0b200 {
+
+namespace {
+
+constexpr int kTile = 64;
+constexpr int kTileK = 16;
+static_assert(kFp8Block % kTileK == 0, "a step along k must not straddle two scales");
+
+__global__ void __launch_bounds__(256) gemm_fp8_simt_kernel(const GemmFp8 p) {
+  grid_dependency_release();
+  grid_dependency_wait();
+  __shared__ float sa[kTileK][kTile + 1];
+  __shared__ float sw[kTileK][kTile + 1];
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const long long m0 = static_cast<long long>(blockIdx.x) * kTile;
+  const int n0 = blockIdx.y * kTile;
+  float acc[4][4] = {};
+  for (int k0 = 0; k0 < p.k; k0 += kTileK) {
+    const int kb = k0 / kFp8Block;
+    for (int i = threadIdx.x; i < kTile * kTileK; i += 256) {
+      const int r = i / kTileK, c = i % kTileK;
+      const long long gm = m0 + r;
+      const int gn = n0 + r, gk = k0 + c;
+      sa[c][r] = (gm < p.m && gk < p.k) ? fp8_value(p.a[gm * p.lda + gk]) * p.a_scale[kb * p.ld_a_scale + gm] : 0.0f;
+      sw[c][r] = (gn < p.n && gk < p.k) ? fp8_value(p.w[gn * p.ldw + gk]) * p.w_scale[(gn / kFp8Block) * p.ld_w_scale + kb] : 0.0f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int kk = 0; kk < kTileK; ++kk) {
+      float av[4], wv[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) av[i] = sa[kk][ty * 4 + i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) wv[j] = sw[kk][tx * 4 + j];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(av[i], wv[j], acc[i][j]);
+      }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const long long gm = m0 + ty * 4 + i;
+    if (gm >= p.m) continue;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int gn = n0 + tx * 4 + j;
+      if (gn >= p.n) continue;
+      const float y = activate_rt(acc[i][j] + (p.bias != nullptr ? __bfloat162float(p.bias[gn]) : 0.0f), p.activation);
+      if (p.out_kind == LC0B200_OUT_F32) reinterpret_cast<float*>(p.out)[gm * p.ldc + gn] = y;
+      else reinterpret_cast<bf16*>(p.out)[gm * p.ldc + gn] = __float2bfloat16_rn(y);
+    }
+  }
+}
+
+}  // namespace
+
+int gemm_fp8_simt(const GemmFp8& g, cudaStream_t stream) {
+  const long long n_tiles = ceil_div_ll(g.n, kTile);
+  if (n_tiles > 65535 || g.m > 0x7FFFFFFFLL) return LC0B200_ERR_UNSUPPORTED;
+  launch_dependent(gemm_fp8_simt_kernel, dim3(static_cast<unsigned>(ceil_div_ll(g.m, kTile)), static_cast<unsigned>(n_tiles)),
+                   dim3(256), 0, stream, g);
+  return launch_status();
+}
+
+int gemm_fp8(const GemmFp8& g, cudaStream_t stream) { return gemm_fp8_simt(g, stream); }
+
+}  // namespace lc0b200

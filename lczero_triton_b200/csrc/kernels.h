@@ -40,6 +40,15 @@ int layer_norm(void* out, const void* in, const void* bias, const void* skip, co
                const void* alpha, long long rows, int width, int activation, int has_skip, float epsilon,
                void* q_out, float* q_scale, cudaStream_t st);
 
+// quantize_fp8.cu
+int quantize_fp8(void* out, float* scale, const void* in, long long rows, int width, int block_rows, long long ld_in,
+                 long long ld_out, long long ld_scale, cudaStream_t st);
+
+// rmsnorm.cu
+int rms_norm(void* out, void* residual, void* q_out, float* q_scale, const void* in, const void* skip, const void* gamma,
+             long long rows, int width, float epsilon, long long ld_in, long long ld_skip, long long ld_out,
+             long long ld_residual, long long ld_q, long long ld_scale, cudaStream_t st);
+
 // attention.cu
 int softmax_64(void* out, const void* qk, const void* smolgen, long long rows, cudaStream_t st);
 int attention(void* out, const void* q, const void* k, const void* v, const void* bias, float scale,
