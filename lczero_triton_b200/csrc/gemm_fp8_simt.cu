@@ -74,6 +74,4 @@ int gemm_fp8_simt(const GemmFp8& g, cudaStream_t stream) {
   return launch_status();
 }
 
-int gemm_fp8(const GemmFp8& g, cudaStream_t stream) { return gemm_fp8_simt(g, stream); }
-
 }  // namespace lc0b200
