@@ -1,0 +1,547 @@
+// Block-scaled e4m3 product on the tensor cores (sm_100a):
+//   out[m,n] = act(bias[n] + sum_b sa[b,m] * sw[n/128,b] * P_b[m,n]),   P_b = the product over 128-block b of k.
+// tcgen05.mma (kind::f8f6f4, f32 accumulation) forms one P_b at a time in tensor memory, overwriting; the epilogue warps
+// read it back, scale it and keep the running sum in registers, so the f32 scales need no restriction and the sum over
+// blocks is a plain fp32 chain in the order of b.  The scale of a block is ONE number per output row and 128 columns,
+// and an epilogue thread owns one row: one fused multiply-add per element and block.
+//
+// gemm_fp8_kernel (many rows): persistent, tiles of 128 x BN per CTA, or 256 x 256 per CTA pair (cta_group::2; each CTA
+// loads its own rows of A and its own half of W with plain TMA loads, none is multicast).  Warp 0 loads (one elected
+// lane), warp 1 issues the MMAs, warps 4 and up are the epilogue: two per TMEM lane quarter for BN >= 128, each with half
+// of the columns.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include "common.cuh"
+#include "fp8.cuh"
+#include "gemm_fp8.h"
+#include "ptx.cuh"
+#include "tensormap.h"
+
+namespace lc0b200 {
+
+namespace {
+
+constexpr int kBM = 128;           // rows of a CTA's tile = TMEM lanes
+constexpr int kRowBytes = 128;     // one swizzle row = one 128-block of k
+constexpr int kMmaK = 32;          // k per tcgen05.mma
+constexpr int kGroupBytes = 32 * kRowBytes;  // staging of 32 rows x 64 bf16 columns, or 32 x 32 f32
+
+template <int CTAS>
+__device__ __forceinline__ void mma_e4m3(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  if (CTAS == 2) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
+        "}\n" ::"r"(tmem_d),
+        "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
+        "}\n" ::"r"(tmem_d),
+        "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  }
+}
+
+// 32 lanes x 16 columns of tensor memory.
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr)
+      : "memory");
+}
+// Waits for this thread's tensor-memory loads; names the registers, so that no use of them can move above it.
+__device__ __forceinline__ void tmem_wait(uint32_t (&v)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                 "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
+               :
+               : "memory");
+}
+
+// Arrival at a barrier of another CTA of the cluster that publishes no memory: it says that tensor-memory loads whose
+// values are in registers are done.  Relaxed, because a release at cluster scope is a memory barrier that waits for
+// everything this thread has in flight, once per k block.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+template <int BN, int CTAS>
+struct Tile {
+  static_assert(CTAS == 1 || (CTAS == 2 && BN == 256), "CTA pairs share 256 x 256 tiles");
+  static constexpr int kABytes = kBM * kRowBytes;
+  static constexpr int kBRows = BN / CTAS;
+  static constexpr int kBBytes = kBRows * kRowBytes;
+  static constexpr int kStageBytes = kABytes + kBBytes;
+  // Block products in flight in tensor memory.  (A 256-wide tile as two half products with barriers of their own, so that
+  // one is handed on while the other is multiplied, was measured slower: 163 us against 139 at 32768 x 1024 x 4096.
+  // MMAs 128 wide are limited by their operand reads from shared memory.)
+  static constexpr int kPartials = BN == 256 ? 2 : 4;
+  static constexpr int kTmemCols = kPartials * BN;  // 512, 512, 256: powers of two
+  static constexpr int kEpilogueWarps = BN >= 128 ? 8 : 4;
+  static constexpr int kCols = BN / (kEpilogueWarps / 4);  // columns per epilogue thread: 128, 64, 64
+  // Four warps in front of the epilogue: loads, MMAs, and two that fetch the scales.
+  static constexpr int kThreads = 128 + 32 * kEpilogueWarps;
+  // 128 running sums a thread do not fit into an even share of the registers (65536 / 384 threads = 168): the first
+  // warpgroup gives some of its own up.  The shares add up to what the block was launched with.
+  static constexpr bool kSplitRegs = kCols == 128;
+  static constexpr int kLaunchRegs = 168, kFrontRegs = 40, kEpilogueRegs = 232;
+  static_assert(128 * kFrontRegs + 256 * kEpilogueRegs <= 384 * kLaunchRegs, "the register shares exceed the launch's");
+  static constexpr int kGroups = kCols / 64;
+  static constexpr int kStagingBytes = kEpilogueWarps * kGroups * kGroupBytes;
+  static constexpr int kBarrierBytes = 512;
+  static constexpr int kScaleSets = 2;                             // k blocks whose scales wait in shared memory
+  static constexpr int kScaleCols = (BN + kFp8Block - 1) / kFp8Block;
+  static constexpr int kScaleBytes = kScaleCols * kBM * 4;         // one product of two scales per row and 128 columns
+  static constexpr int kFixedBytes = kStagingBytes + kBarrierBytes + kScaleSets * kScaleBytes;
+  static constexpr int kFit = (227 * 1024 - kFixedBytes) / kStageBytes;
+  static constexpr int kStages = kFit > 8 ? 8 : kFit;
+  static_assert(kStages >= 3, "pipeline too shallow");
+  static constexpr int kSmemBytes = kStages * kStageBytes + kFixedBytes;
+};
+
+struct FpParams {
+  GemmFp8 g;
+  int tma_store;  // bf16 result with a base, pitch and width that a tensor map can store
+  unsigned int* status;
+};
+
+// Columns that the MMAs of the tile at tile_n0 cover: a ragged last tile costs its own width rounded up to 32.
+template <int BN>
+__device__ __forceinline__ int mma_width(int n, int tile_n0) {
+  const int left = n - tile_n0;
+  return left >= BN ? BN : ((left + 31) & ~31);
+}
+
+// Bias and activation of 32 columns from col0 on; columns past the matrix edge get no bias (they are not stored).
+__device__ __forceinline__ void finish32(float (&y)[32], const GemmFp8& g, int col0) {
+  if (g.bias != nullptr) {
+    if (col0 + 32 <= g.n && aligned16_dev(g.bias)) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint4 raw = __ldg(reinterpret_cast<const uint4*>(g.bias + col0) + i);
+        const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 b = unpack_bf16x2(words[j]);
+          y[8 * i + 2 * j] += b.x;
+          y[8 * i + 2 * j + 1] += b.y;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) y[j] += col0 + j < g.n ? __bfloat162float(g.bias[col0 + j]) : 0.0f;
+    }
+  }
+  // The activation is uniform for the launch: one branch per chunk, not per element.
+  if (g.activation == LC0B200_ACT_MISH) {
+    mish32(y);
+  } else if (g.activation == LC0B200_ACT_RELU) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) y[j] = y[j] < 0.0f ? 0.0f : y[j];  // NaN stays
+  } else if (g.activation == LC0B200_ACT_SWISH) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) y[j] = act_swish(y[j]);
+  }
+}
+
+template <int BN, int CTAS>
+__global__ void __launch_bounds__(Tile<BN, CTAS>::kThreads, 1)
+gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
+                const __grid_constant__ CUtensorMap map_out, const FpParams p) {
+  using T = Tile<BN, CTAS>;
+  constexpr int kStages = T::kStages;
+  constexpr int kPartials = T::kPartials;
+  constexpr int kTileM = kBM * CTAS;
+
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t smem_base = ptx::smem_u32(smem_raw);
+  const uint32_t smem_a = smem_base;
+  const uint32_t smem_b = smem_base + kStages * T::kABytes;
+  const uint32_t staging_base = smem_base + kStages * T::kStageBytes;
+  const uint32_t bar_base = staging_base + T::kStagingBytes;
+  const uint32_t bar_full = bar_base;                                   // [kStages] (leader CTA's are used)
+  const uint32_t bar_empty = bar_base + 8 * kStages;                    // [kStages]
+  const uint32_t bar_part_full = bar_base + 16 * kStages;               // [kPartials]
+  const uint32_t bar_part_empty = bar_part_full + 8 * kPartials;        // [kPartials] (leader CTA's are used)
+  const uint32_t bar_scale_full = bar_part_empty + 8 * kPartials;       // [kScaleSets]
+  const uint32_t bar_scale_empty = bar_scale_full + 8 * T::kScaleSets;  // [kScaleSets]
+  const uint32_t tmem_slot = bar_scale_empty + 8 * T::kScaleSets;
+  const uint32_t scale_base = bar_base + T::kBarrierBytes;              // [kScaleSets][kScaleCols][kBM] f32
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem_raw + (tmem_slot + 4 - smem_base));
+  static_assert(16 * kStages + 16 * kPartials + 16 * T::kScaleSets + 8 <= T::kBarrierBytes, "barrier area too small");
+  grid_dependency_release();
+  if ((smem_base & 1023u) != 0u) {  // never seen; refuse loudly rather than mis-swizzle
+    if (threadIdx.x == 0 && atomicCAS(&p.status[0], 0u, kDeviceSmemMisaligned) == 0u) p.status[1] = smem_base;
+    return;
+  }
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = (CTAS == 2) ? ptx::cluster_ctarank() : 0u;  // rank 0 leads: issues the MMAs, owns the barriers
+  const uint32_t group = blockIdx.x / CTAS;
+  const uint32_t num_groups = gridDim.x / CTAS;
+  const GemmFp8& g = p.g;
+  const int n_tiles = (g.n + BN - 1) / BN;
+  const long long num_tiles = ceil_div_ll(g.m, kTileM) * n_tiles;
+  const int k_blocks = (g.k + kFp8Block - 1) / kFp8Block;
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int s = 0; s < kStages; ++s) {
+      ptx::mbar_init(bar_full + 8 * s, 1);
+      ptx::mbar_init(bar_empty + 8 * s, 1);
+    }
+    for (int a = 0; a < kPartials; ++a) {
+      ptx::mbar_init(bar_part_full + 8 * a, 1);
+      ptx::mbar_init(bar_part_empty + 8 * a, T::kEpilogueWarps * CTAS);
+    }
+    for (int i = 0; i < T::kScaleSets; ++i) {
+      ptx::mbar_init(bar_scale_full + 8 * i, 1);
+      ptx::mbar_init(bar_scale_empty + 8 * i, T::kEpilogueWarps);
+    }
+    ptx::mbar_init_fence();
+    ptx::prefetch_tensormap(&map_a);
+    ptx::prefetch_tensormap(&map_w);
+    if (p.tma_store) ptx::prefetch_tensormap(&map_out);
+  }
+  if (warp == 1) {
+    if (CTAS == 2) {
+      ptx::tmem_alloc_pair(tmem_slot, T::kTmemCols);
+      ptx::tmem_relinquish_pair();
+    } else {
+      ptx::tmem_alloc(tmem_slot, T::kTmemCols);
+      ptx::tmem_relinquish();
+    }
+  }
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  if (CTAS == 2) ptx::cluster_sync();  // the peer's barriers exist before anything signals them
+  ptx::tc_fence_after_sync();
+  uint32_t tmem_base;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem_base) : "r"(tmem_slot));
+  grid_dependency_wait();
+
+  if (warp < 4) {
+    if (T::kSplitRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(T::kFrontRegs));
+  if (warp == 0) {
+    // ------------------------------------------------------------ loads: the warp follows the loop, one lane issues
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (long long tile = group; tile < num_tiles && ok; tile += num_groups) {
+      const int m0 = static_cast<int>(tile / n_tiles) * kTileM + static_cast<int>(rank) * kBM;
+      const int tile_n0 = static_cast<int>(tile % n_tiles) * BN;
+      // A pair splits the weight tile's rows between its CTAs.
+      const int n0 = tile_n0 + static_cast<int>(rank) * (mma_width<BN>(g.n, tile_n0) / CTAS);
+      for (int kb = 0; kb < k_blocks; ++kb) {
+        ok = ptx::mbar_wait(bar_empty + 8 * stage, phase ^ 1u, abort_flag, p.status, 0x1100u + stage);
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        if (!ok) break;
+        if (ptx::elect_one()) {
+          const uint32_t full = (CTAS == 2) ? ptx::map_to_cta(bar_full + 8 * stage, 0u) : bar_full + 8 * stage;
+          if (rank == 0) ptx::mbar_expect_tx(bar_full + 8 * stage, T::kStageBytes * CTAS);
+          ptx::tma_load_2d<CTAS>(smem_a + stage * T::kABytes, &map_a, kb * kFp8Block, m0, full);
+          ptx::tma_load_2d<CTAS>(smem_b + stage * T::kBBytes, &map_w, kb * kFp8Block, n0, full);
+        }
+        if (++stage == kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMAs (leader CTA only): one partial per k block
+    if (rank == 0) {
+      int stage = 0, part = 0;
+      uint32_t phase = 0, part_phase = 0;
+      bool ok = true;
+      for (long long tile = group; tile < num_tiles && ok; tile += num_groups) {
+        const int tile_n0 = static_cast<int>(tile % n_tiles) * BN;
+        const uint32_t idesc = ptx::instr_desc(1u, 0u, 0u, static_cast<uint32_t>(kTileM),
+                                               static_cast<uint32_t>(mma_width<BN>(g.n, tile_n0)));
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          ok = ptx::mbar_wait(bar_part_empty + 8 * part, part_phase ^ 1u, abort_flag, p.status, 0x1200u + part);
+          ok = ok && ptx::mbar_wait(bar_full + 8 * stage, phase, abort_flag, p.status, 0x1300u + stage);
+          ok = __all_sync(0xFFFFFFFFu, ok);
+          if (!ok) break;
+          ptx::tc_fence_after_sync();
+          if (ptx::elect_one()) {
+            const uint32_t a_addr = smem_a + stage * T::kABytes;
+            const uint32_t b_addr = smem_b + stage * T::kBBytes;
+#pragma unroll
+            for (int j = 0; j < kFp8Block / kMmaK; ++j) {
+              mma_e4m3<CTAS>(tmem_base + part * BN, ptx::smem_desc_sw128(a_addr + j * kMmaK, 16, 1024),
+                             ptx::smem_desc_sw128(b_addr + j * kMmaK, 16, 1024), idesc, j > 0 ? 1u : 0u);
+            }
+            ptx::tc_commit<CTAS>(bar_empty + 8 * stage);
+            ptx::tc_commit<CTAS>(bar_part_full + 8 * part);
+          }
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+          if (++part == kPartials) {
+            part = 0;
+            part_phase ^= 1u;
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ scales: a_scale[row] * w_scale of each k block
+    // Two warps take the k blocks in turn, one set of shared memory each.  (Epilogue warps that fetched their own were
+    // slower, 176 us against 137 at 32768 x 1024 x 4096 in the worst schedule: a wait for tensor memory may then
+    // also wait for a global load.)
+    const int set = warp - 2;
+    const uint32_t dst = scale_base + set * T::kScaleBytes;
+    uint32_t phase = 0;
+    long long tile = group;
+    int kb = set;
+    while (true) {
+      while (kb >= k_blocks) {
+        kb -= k_blocks;
+        tile += num_groups;
+      }
+      if (tile >= num_tiles) break;
+      const long long row0 = (tile / n_tiles) * kTileM + rank * kBM + lane;
+      const int column = static_cast<int>(tile % n_tiles) * BN;
+      float a[4], w[T::kScaleCols];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] = row0 + 32 * i < g.m ? __ldg(g.a_scale + kb * g.ld_a_scale + row0 + 32 * i) : 0.0f;
+#pragma unroll
+      for (int h = 0; h < T::kScaleCols; ++h) {
+        const int n0 = column + h * kFp8Block;
+        w[h] = n0 < g.n ? __ldg(g.w_scale + (n0 / kFp8Block) * g.ld_w_scale + kb) : 0.0f;
+      }
+      bool ok = ptx::mbar_wait(bar_scale_empty + 8 * set, phase ^ 1u, abort_flag, p.status, 0x1500u + set);
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      if (!ok) break;
+#pragma unroll
+      for (int h = 0; h < T::kScaleCols; ++h) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst + (h * kBM + 32 * i + lane) * 4), "f"(a[i] * w[h]) : "memory");
+        }
+      }
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(bar_scale_full + 8 * set);
+      phase ^= 1u;
+      kb += T::kScaleSets;
+    }
+    __syncwarp();
+  }
+  } else {
+    if (T::kSplitRegs) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(T::kEpilogueRegs));
+    // ------------------------------------------------------------ epilogue: scale and sum the partials, then store
+    const int ew = warp - 4;
+    const int quarter = warp & 3;  // TMEM lane quarter this warp may read
+    const int half = ew >> 2;
+    const uint32_t staging = staging_base + ew * T::kGroups * kGroupBytes;
+    const uint32_t tmem_row = tmem_base + half * T::kCols + (static_cast<uint32_t>(quarter * 32) << 16);
+    int part = 0;
+    uint32_t part_phase = 0;
+    bool ok = true;
+    auto row_of = [&](long long tile) { return (tile / n_tiles) * kTileM + rank * kBM + quarter * 32 + lane; };
+    auto column_of = [&](long long tile) { return static_cast<int>(tile % n_tiles) * BN + half * T::kCols; };
+    int set = 0;
+    uint32_t set_phase = 0;
+    const uint32_t my_scale = scale_base + ((half * T::kCols / kFp8Block) * kBM + quarter * 32 + lane) * 4;
+    for (long long tile = group; tile < num_tiles && ok; tile += num_groups) {
+      const long long row = row_of(tile);
+      const int n0 = column_of(tile);
+      float acc[T::kCols];
+#pragma unroll
+      for (int i = 0; i < T::kCols; ++i) acc[i] = 0.0f;
+      for (int kb = 0; kb < k_blocks; ++kb) {
+        ok = ptx::mbar_wait(bar_scale_full + 8 * set, set_phase, abort_flag, p.status, 0x1600u + set);
+        if (!ok) break;
+        float scale;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(scale) : "r"(my_scale + set * T::kScaleBytes) : "memory");
+        ok = ptx::mbar_wait(bar_part_full + 8 * part, part_phase, abort_flag, p.status, 0x1400u + part);
+        if (!ok) break;
+        ptx::tc_fence_after_sync();
+        const uint32_t taddr = tmem_row + part * BN;
+        // Sixteen columns at a time, the next sixteen on their way while these are added.  (Measured at 32768 x 1024
+        // x 4096: 32 at a time is 9 % slower, packed pairs of multiply-adds 3 %.)  Columns past the matrix edge hold
+        // anything and are not stored.
+        uint32_t v[2][16];
+        tmem_ld_32x16(taddr, v[0]);
+#pragma unroll
+        for (int c = 0; c < T::kCols / 16; ++c) {
+          tmem_wait(v[c & 1]);
+          if (c + 1 < T::kCols / 16) {
+            tmem_ld_32x16(taddr + 16 * (c + 1), v[(c + 1) & 1]);
+          } else {
+            // The last columns and the scale are in registers: partial and scales go back to the warps that fill them.
+            ptx::tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) {
+              if (CTAS == 2) mbar_arrive_cluster_relaxed(ptx::map_to_cta(bar_part_empty + 8 * part, 0u));
+              else ptx::mbar_arrive(bar_part_empty + 8 * part);
+              ptx::mbar_arrive(bar_scale_empty + 8 * set);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j) acc[c * 16 + j] = fmaf(__uint_as_float(v[c & 1][j]), scale, acc[c * 16 + j]);
+        }
+        if (++part == kPartials) {
+          part = 0;
+          part_phase ^= 1u;
+        }
+        if (++set == T::kScaleSets) {
+          set = 0;
+          set_phase ^= 1u;
+        }
+      }
+      if (!ok) break;
+      // ---- bias, activation, store
+      if (p.tma_store) {
+        if (lane == 0) ptx::bulk_wait_read<0>();  // the staging buffers are free once the last tile's stores have read them
+        __syncwarp();
+      }
+#pragma unroll
+      for (int c = 0; c < T::kCols / 32; ++c) {
+        const int col0 = n0 + 32 * c;
+        float y[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) y[j] = acc[c * 32 + j];
+        if (col0 < g.n) {
+          finish32(y, g, col0);
+          if (p.tma_store) {
+            // Row `lane` of the group's 32 x 128-byte buffer, 16-byte chunk i at i ^ (lane & 7): the 128-byte swizzle.
+            const uint32_t row_addr = staging + (c >> 1) * kGroupBytes + lane * kRowBytes;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              ptx::st_shared_v4(row_addr + ((((c & 1) * 4 + i) ^ (lane & 7)) << 4), pack_bf16x2(y[8 * i], y[8 * i + 1]),
+                                pack_bf16x2(y[8 * i + 2], y[8 * i + 3]), pack_bf16x2(y[8 * i + 4], y[8 * i + 5]),
+                                pack_bf16x2(y[8 * i + 6], y[8 * i + 7]));
+            }
+          } else {
+            // f32 results and rows a tensor map cannot address: turn the 32 x 32 block in shared memory (element c of
+            // row r at c ^ r, no bank conflicts either way) and write whole rows, 32 neighbouring elements a store.
+            float* block = reinterpret_cast<float*>(smem_raw + (staging - smem_base));
+#pragma unroll
+            for (int j = 0; j < 32; ++j) block[lane * 32 + (j ^ lane)] = y[j];
+            __syncwarp();
+            const int rows = static_cast<int>(min(static_cast<long long>(32), g.m - (row - lane)));
+            if (col0 + lane < g.n) {
+              for (int r = 0; r < rows; ++r) {
+                const float value = block[r * 32 + (lane ^ r)];
+                const long long at = (row - lane + r) * g.ldc + col0 + lane;
+                if (g.out_kind == LC0B200_OUT_F32) reinterpret_cast<float*>(g.out)[at] = value;
+                else reinterpret_cast<bf16*>(g.out)[at] = __float2bfloat16_rn(value);
+              }
+            }
+            __syncwarp();
+          }
+        }
+      }
+      if (p.tma_store && n0 < g.n) {
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+#pragma unroll
+          for (int i = 0; i < T::kGroups; ++i) {
+            if (n0 + 64 * i < g.n) {
+              ptx::tma_store_2d(&map_out, staging + i * kGroupBytes, n0 + 64 * i, static_cast<int>(row));
+            }
+          }
+          ptx::bulk_commit();
+        }
+      }
+    }
+    if (p.tma_store && lane == 0) ptx::bulk_wait_read<0>();  // staging must outlive the last store's read
+    __syncwarp();
+  }
+
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  if (CTAS == 2) ptx::cluster_sync();  // neither CTA leaves while the other can signal its barriers or read its memory
+  if (warp == 1) {
+    ptx::tc_fence_after_sync();
+    if (CTAS == 2) ptx::tmem_dealloc_pair(tmem_base, T::kTmemCols);
+    else ptx::tmem_dealloc(tmem_base, T::kTmemCols);
+  }
+}
+
+bool make_map(CUtensorMap* map, const void* base, int elem_bytes, long long rows, long long cols, long long pitch,
+              int box_rows, int box_cols) {
+  return make_tensormap_2d(map, base, elem_bytes, rows, cols, pitch, box_rows, box_cols, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <int BN, int CTAS>
+int launch(const GemmFp8& g, cudaStream_t stream) {
+  using T = Tile<BN, CTAS>;
+  CUtensorMap map_a, map_w;
+  if (!make_map(&map_a, g.a, 1, g.m, g.k, g.lda, kBM, kFp8Block)) return LC0B200_ERR_CUDA;
+  if (!make_map(&map_w, g.w, 1, g.n, g.k, g.ldw, T::kBRows, kFp8Block)) return LC0B200_ERR_CUDA;
+  FpParams p;
+  p.g = g;
+  // (A TMA store clips a row at whole 16 bytes: with n not a multiple of 8 it would write into the pitch.)
+  p.tma_store = g.out_kind == LC0B200_OUT_BF16 && aligned16(g.out) && (g.ldc % 8) == 0 && (g.n % 8) == 0;
+  CUtensorMap map_out = map_a;  // placeholder when unused
+  if (p.tma_store && !make_map(&map_out, g.out, 2, g.m, g.n, g.ldc, 32, 64)) return LC0B200_ERR_CUDA;
+  p.status = device_status_words();
+  if (p.status == nullptr) return LC0B200_ERR_CUDA;
+  auto kernel = gemm_fp8_kernel<BN, CTAS>;
+  static PerDeviceOnce smem_opt_in;  // per instantiation
+  if (allow_dynamic_smem(smem_opt_in, kernel, T::kSmemBytes) != LC0B200_OK) return LC0B200_ERR_CUDA;
+  if (T::kSplitRegs) {
+    // A register split that asks for more than the launch has would wait for ever.
+    static const int launch_regs = [](auto k) {
+      cudaFuncAttributes attributes;
+      return cudaFuncGetAttributes(&attributes, k) == cudaSuccess ? attributes.numRegs : 0;
+    }(kernel);
+    if (launch_regs < T::kLaunchRegs) return LC0B200_ERR_UNSUPPORTED;
+  }
+  const long long tiles = ceil_div_ll(g.m, kBM * CTAS) * ceil_div_ll(g.n, BN);
+  const long long max_groups = sm_count() / CTAS;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((tiles < max_groups ? tiles : max_groups) * CTAS));
+  cfg.blockDim = dim3(T::kThreads);
+  cfg.dynamicSmemBytes = T::kSmemBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0] = dependent_launch_attribute();
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = CTAS;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = CTAS == 2 ? 2 : 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, map_a, map_w, map_out, p) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return LC0B200_ERR_CUDA;
+  }
+  return LC0B200_OK;
+}
+
+}  // namespace
+
+int gemm_fp8(const GemmFp8& given, cudaStream_t stream) {
+  GemmFp8 g = given;
+  // The pitch of a single row says nothing; make it one that TMA takes.
+  if (g.m == 1) g.lda = ceil_div_ll(g.k, 16) * 16;
+  if (g.n == 1) g.ldw = ceil_div_ll(g.k, 16) * 16;
+  if (!aligned16(g.a) || !aligned16(g.w) || (g.lda % 16) != 0 || (g.ldw % 16) != 0) return gemm_fp8_simt(g, stream);
+  // The widest tile that still gives most SMs one.
+  const long long enough = sm_count() * 3LL / 5;
+  if (2 * ceil_div_ll(g.m, 2 * kBM) * ceil_div_ll(g.n, 256) >= enough) return launch<256, 2>(g, stream);
+  if (ceil_div_ll(g.m, kBM) * ceil_div_ll(g.n, 128) >= enough) return launch<128, 1>(g, stream);
+  return launch<64, 1>(g, stream);
+}
+
+}  // namespace lc0b200

@@ -358,6 +358,19 @@ def test_gemm_nan_stays_in_its_row_and_column(ops, m) -> None:
     assert torch.equal(out[rows][:, columns], clean[rows][:, columns])
 
 
+@pytest.mark.parametrize("activation", ["mish", "relu", "swish"])
+@pytest.mark.parametrize("m, pitch", [(3, 256), (3, 257), (70, 256), (300, 256)])
+def test_gemm_nan_passes_the_activation(ops, activation, m, pitch) -> None:
+    n, k = 130, 256
+    a, a_scale, w, w_scale = _operands(33, m, n, k)
+    clean, out = torch.empty((m, n), device="cuda"), torch.empty((m, n), device="cuda")
+    ops.gemm_fp8(clean, _placed(a, pitch), a_scale, w, w_scale, activation=activation)
+    a.view(torch.uint8)[1, 7] = 0x7F
+    ops.gemm_fp8(out, _placed(a, pitch), a_scale, w, w_scale, activation=activation)
+    assert bool(torch.isnan(out[1]).all())
+    assert torch.equal(out[0], clean[0]) and torch.equal(out[2:], clean[2:])
+
+
 def test_gemm_scales_of_slices(ops) -> None:
     """Rows of a larger batch: codes, scales and results are views with the batch's pitches."""
     m, n, k = 500, 192, 512
