@@ -50,23 +50,43 @@ __device__ __forceinline__ void mma_e4m3(uint32_t tmem_d, uint64_t desc_a, uint6
   }
 }
 
-// 32 lanes x 16 columns of tensor memory.
-__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&v)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-      : "r"(taddr)
-      : "memory");
-}
 // Waits for this thread's tensor-memory loads; names the registers, so that no use of them can move above it.
-__device__ __forceinline__ void tmem_wait(uint32_t (&v)[16]) {
+__device__ __forceinline__ void tmem_wait(uint32_t (&v)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
-                 "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
+                 "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]),
+                 "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]),
+                 "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
                :
                : "memory");
+}
+
+// A look at a barrier that never suspends.
+__device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "}\n"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+
+__device__ __forceinline__ uint64_t pack_f32x2(uint32_t lo, uint32_t hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack_f32x2(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+// acc += a * b, both halves.
+__device__ __forceinline__ void fma_f32x2(uint64_t& acc, uint64_t a, uint64_t b) {
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b));
 }
 
 // Arrival at a barrier of another CTA of the cluster that publishes no memory: it says that tensor-memory loads whose
@@ -100,10 +120,9 @@ struct Tile {
   static constexpr int kGroups = kCols / 64;
   static constexpr int kStagingBytes = kEpilogueWarps * kGroups * kGroupBytes;
   static constexpr int kBarrierBytes = 512;
-  static constexpr int kScaleSets = 2;                             // k blocks whose scales wait in shared memory
   static constexpr int kScaleCols = (BN + kFp8Block - 1) / kFp8Block;
   static constexpr int kScaleBytes = kScaleCols * kBM * 4;         // one product of two scales per row and 128 columns
-  static constexpr int kFixedBytes = kStagingBytes + kBarrierBytes + kScaleSets * kScaleBytes;
+  static constexpr int kFixedBytes = kStagingBytes + kBarrierBytes + kPartials * kScaleBytes;
   static constexpr int kFit = (227 * 1024 - kFixedBytes) / kStageBytes;
   static constexpr int kStages = kFit > 8 ? 8 : kFit;
   static_assert(kStages >= 3, "pipeline too shallow");
@@ -172,14 +191,13 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
   const uint32_t bar_base = staging_base + T::kStagingBytes;
   const uint32_t bar_full = bar_base;                                   // [kStages] (leader CTA's are used)
   const uint32_t bar_empty = bar_base + 8 * kStages;                    // [kStages]
-  const uint32_t bar_part_full = bar_base + 16 * kStages;               // [kPartials]
+  const uint32_t bar_part_full = bar_base + 16 * kStages;               // [kPartials] product and scales are there
   const uint32_t bar_part_empty = bar_part_full + 8 * kPartials;        // [kPartials] (leader CTA's are used)
-  const uint32_t bar_scale_full = bar_part_empty + 8 * kPartials;       // [kScaleSets]
-  const uint32_t bar_scale_empty = bar_scale_full + 8 * T::kScaleSets;  // [kScaleSets]
-  const uint32_t tmem_slot = bar_scale_empty + 8 * T::kScaleSets;
-  const uint32_t scale_base = bar_base + T::kBarrierBytes;              // [kScaleSets][kScaleCols][kBM] f32
+  const uint32_t bar_scale_empty = bar_part_empty + 8 * kPartials;      // [kPartials]
+  const uint32_t tmem_slot = bar_scale_empty + 8 * kPartials;
+  const uint32_t scale_base = bar_base + T::kBarrierBytes;              // [kPartials][kScaleCols][kBM] f32
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem_raw + (tmem_slot + 4 - smem_base));
-  static_assert(16 * kStages + 16 * kPartials + 16 * T::kScaleSets + 8 <= T::kBarrierBytes, "barrier area too small");
+  static_assert(16 * kStages + 24 * kPartials + 8 <= T::kBarrierBytes, "barrier area too small");
   grid_dependency_release();
   if ((smem_base & 1023u) != 0u) {  // never seen; refuse loudly rather than mis-swizzle
     if (threadIdx.x == 0 && atomicCAS(&p.status[0], 0u, kDeviceSmemMisaligned) == 0u) p.status[1] = smem_base;
@@ -203,12 +221,9 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       ptx::mbar_init(bar_empty + 8 * s, 1);
     }
     for (int a = 0; a < kPartials; ++a) {
-      ptx::mbar_init(bar_part_full + 8 * a, 1);
+      ptx::mbar_init(bar_part_full + 8 * a, 2);  // the MMAs' completion and a scale warp
       ptx::mbar_init(bar_part_empty + 8 * a, T::kEpilogueWarps * CTAS);
-    }
-    for (int i = 0; i < T::kScaleSets; ++i) {
-      ptx::mbar_init(bar_scale_full + 8 * i, 1);
-      ptx::mbar_init(bar_scale_empty + 8 * i, T::kEpilogueWarps);
+      ptx::mbar_init(bar_scale_empty + 8 * a, T::kEpilogueWarps);
     }
     ptx::mbar_init_fence();
     ptx::prefetch_tensormap(&map_a);
@@ -302,14 +317,14 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     __syncwarp();
   } else {
     // ------------------------------------------------------------ scales: a_scale[row] * w_scale of each k block
-    // Two warps take the k blocks in turn, one set of shared memory each.  (Epilogue warps that fetched their own were
-    // slower, 176 us against 137 at 32768 x 1024 x 4096 in the worst schedule: a wait for tensor memory may then
-    // also wait for a global load.)
-    const int set = warp - 2;
-    const uint32_t dst = scale_base + set * T::kScaleBytes;
+    // Two warps take the k blocks in turn; the scales of a block wait in shared memory beside its partial, behind the
+    // same barrier.  (Epilogue warps that fetched their own were slower, 176 us against 137 at 32768 x 1024 x 4096 in the
+    // worst schedule: a wait for tensor memory may then also wait for a global load.)
+    const int first = warp - 2;
+    int part = first;
     uint32_t phase = 0;
     long long tile = group;
-    int kb = set;
+    int kb = first;
     while (true) {
       while (kb >= k_blocks) {
         kb -= k_blocks;
@@ -326,20 +341,24 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         const int n0 = column + h * kFp8Block;
         w[h] = n0 < g.n ? __ldg(g.w_scale + (n0 / kFp8Block) * g.ld_w_scale + kb) : 0.0f;
       }
-      bool ok = ptx::mbar_wait(bar_scale_empty + 8 * set, phase ^ 1u, abort_flag, p.status, 0x1500u + set);
+      bool ok = ptx::mbar_wait(bar_scale_empty + 8 * part, phase ^ 1u, abort_flag, p.status, 0x1500u + part);
       ok = __all_sync(0xFFFFFFFFu, ok);
       if (!ok) break;
 #pragma unroll
       for (int h = 0; h < T::kScaleCols; ++h) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst + (h * kBM + 32 * i + lane) * 4), "f"(a[i] * w[h]) : "memory");
+          asm volatile("st.shared.f32 [%0], %1;" ::"r"(scale_base + part * T::kScaleBytes + (h * kBM + 32 * i + lane) * 4), "f"(a[i] * w[h]) : "memory");
         }
       }
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(bar_scale_full + 8 * set);
-      phase ^= 1u;
-      kb += T::kScaleSets;
+      if (lane == 0) ptx::mbar_arrive(bar_part_full + 8 * part);
+      part += 2;
+      if (part >= kPartials) {
+        part = first;
+        phase ^= 1u;
+      }
+      kb += 2;
     }
     __syncwarp();
   }
@@ -356,55 +375,59 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     bool ok = true;
     auto row_of = [&](long long tile) { return (tile / n_tiles) * kTileM + rank * kBM + quarter * 32 + lane; };
     auto column_of = [&](long long tile) { return static_cast<int>(tile % n_tiles) * BN + half * T::kCols; };
-    int set = 0;
-    uint32_t set_phase = 0;
     const uint32_t my_scale = scale_base + ((half * T::kCols / kFp8Block) * kBM + quarter * 32 + lane) * 4;
     for (long long tile = group; tile < num_tiles && ok; tile += num_groups) {
       const long long row = row_of(tile);
       const int n0 = column_of(tile);
-      float acc[T::kCols];
+      // Running sums as packed pairs of fp32: one packed multiply-add for two columns.
+      constexpr int kChunks = T::kCols / 32;
+      static_assert(kChunks % 2 == 0, "a block's first columns go to the first buffer");
+      uint64_t acc[T::kCols / 2];
 #pragma unroll
-      for (int i = 0; i < T::kCols; ++i) acc[i] = 0.0f;
-      for (int kb = 0; kb < k_blocks; ++kb) {
-        ok = ptx::mbar_wait(bar_scale_full + 8 * set, set_phase, abort_flag, p.status, 0x1600u + set);
-        if (!ok) break;
-        float scale;
-        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(scale) : "r"(my_scale + set * T::kScaleBytes) : "memory");
-        ok = ptx::mbar_wait(bar_part_full + 8 * part, part_phase, abort_flag, p.status, 0x1400u + part);
-        if (!ok) break;
+      for (int i = 0; i < T::kCols / 2; ++i) acc[i] = 0ull;
+      // 32 columns at a time: while they are added, the next 32 are on their way, across the k blocks too (a partial is
+      // handed back, and the next one's first columns asked for, before the last additions).  Columns past the matrix
+      // edge hold anything and are not stored.
+      float scale = 0.0f, next_scale = 0.0f;
+      uint32_t v[2][32];
+      bool ready = false;
+      auto begin_block = [&](float& block_scale) {
+        if (!ready) ok = ptx::mbar_wait(bar_part_full + 8 * part, part_phase, abort_flag, p.status, 0x1400u + part);
+        if (!ok) return;
         ptx::tc_fence_after_sync();
-        const uint32_t taddr = tmem_row + part * BN;
-        // Sixteen columns at a time, the next sixteen on their way while these are added.  (Measured at 32768 x 1024
-        // x 4096: 32 at a time is 9 % slower, packed pairs of multiply-adds 3 %.)  Columns past the matrix edge hold
-        // anything and are not stored.
-        uint32_t v[2][16];
-        tmem_ld_32x16(taddr, v[0]);
-#pragma unroll
-        for (int c = 0; c < T::kCols / 16; ++c) {
-          tmem_wait(v[c & 1]);
-          if (c + 1 < T::kCols / 16) {
-            tmem_ld_32x16(taddr + 16 * (c + 1), v[(c + 1) & 1]);
-          } else {
-            // The last columns and the scale are in registers: partial and scales go back to the warps that fill them.
-            ptx::tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) {
-              if (CTAS == 2) mbar_arrive_cluster_relaxed(ptx::map_to_cta(bar_part_empty + 8 * part, 0u));
-              else ptx::mbar_arrive(bar_part_empty + 8 * part);
-              ptx::mbar_arrive(bar_scale_empty + 8 * set);
-            }
-          }
-#pragma unroll
-          for (int j = 0; j < 16; ++j) acc[c * 16 + j] = fmaf(__uint_as_float(v[c & 1][j]), scale, acc[c * 16 + j]);
-        }
+        ptx::tmem_ld_32x32(tmem_row + part * BN, v[0]);
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(block_scale) : "r"(my_scale + part * T::kScaleBytes) : "memory");
+      };
+      begin_block(scale);
+      for (int kb = 0; kb < k_blocks && ok; ++kb) {
+        const uint64_t scale2 = pack_f32x2(__float_as_uint(scale), __float_as_uint(scale));
+        const int this_part = part;
         if (++part == kPartials) {
           part = 0;
           part_phase ^= 1u;
         }
-        if (++set == T::kScaleSets) {
-          set = 0;
-          set_phase ^= 1u;
+        ready = false;
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+          tmem_wait(v[c & 1]);
+          if (c + 1 < kChunks) {
+            ptx::tmem_ld_32x32(tmem_row + this_part * BN + 32 * (c + 1), v[(c + 1) & 1]);
+            // Look at the next partial's barrier while there is work to hide the look behind.
+            if (c + 2 == kChunks && kb + 1 < k_blocks) ready = mbar_test_wait(bar_part_full + 8 * part, part_phase);
+          } else {
+            ptx::tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) {
+              if (CTAS == 2) mbar_arrive_cluster_relaxed(ptx::map_to_cta(bar_part_empty + 8 * this_part, 0u));
+              else ptx::mbar_arrive(bar_part_empty + 8 * this_part);
+              ptx::mbar_arrive(bar_scale_empty + 8 * this_part);
+            }
+            if (kb + 1 < k_blocks) begin_block(next_scale);
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j) fma_f32x2(acc[c * 16 + j], pack_f32x2(v[c & 1][2 * j], v[c & 1][2 * j + 1]), scale2);
         }
+        scale = next_scale;
       }
       if (!ok) break;
       // ---- bias, activation, store
@@ -417,7 +440,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         const int col0 = n0 + 32 * c;
         float y[32];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) y[j] = acc[c * 32 + j];
+        for (int j = 0; j < 16; ++j) unpack_f32x2(acc[c * 16 + j], y[2 * j], y[2 * j + 1]);
         if (col0 < g.n) {
           finish32(y, g, col0);
           if (p.tma_store) {
