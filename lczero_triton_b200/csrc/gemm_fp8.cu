@@ -61,6 +61,30 @@ __device__ __forceinline__ void tmem_wait(uint32_t (&v)[32]) {
                : "memory");
 }
 
+__device__ __forceinline__ void tmem_wait(uint32_t (&v)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                 "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_wait(uint32_t (&v)[64]) {
+  tmem_wait(*reinterpret_cast<uint32_t(*)[32]>(&v[0]));
+  tmem_wait(*reinterpret_cast<uint32_t(*)[32]>(&v[32]));
+}
+// 32 lanes x 16 / 32 / 64 columns of tensor memory.
+__device__ __forceinline__ void tmem_ld_columns(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_columns(uint32_t taddr, uint32_t (&v)[32]) { ptx::tmem_ld_32x32(taddr, v); }
+__device__ __forceinline__ void tmem_ld_columns(uint32_t taddr, uint32_t (&v)[64]) { ptx::tmem_ld_32x64(taddr, v); }
+
 // A look at a barrier that never suspends.
 __device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity) {
   uint32_t done;
@@ -500,6 +524,255 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
   }
 }
 
+// ---------------------------------------------------------------- few rows
+//
+// At most 64 rows of A: the weight's bytes are the work, and a 128-row tile of A would be mostly padding.  So the roles
+// are turned round: 128 weight rows are the M side of the MMA, the tokens its N side (NT = 16, 32 or 64 columns), and
+// out^T comes out: an epilogue thread owns one weight row, a block's scales are one product per token.  The k blocks of a
+// tile are split over the CTAs of a cluster, so that a layer of a few tiles still pulls on the memory of most SMs; their
+// sums meet in distributed shared memory, added in the order of the CTAs (the same bits every time).  Half of an SM's
+// shared memory per CTA, so that the next tile's loads can start while a CTA finishes.
+template <int NT>
+struct Few {
+  static constexpr int kWBytes = kBM * kRowBytes;
+  static constexpr int kStageBytes = kWBytes + NT * kRowBytes;
+  static constexpr int kPartials = 4;
+  static constexpr int kTmemCols = kPartials * NT;  // 64, 128, 256
+  static constexpr int kThreads = 256;              // warps: loads, MMAs, two for scales, four epilogue
+  static constexpr int kBarrierBytes = 512;
+  static constexpr int kScaleBytes = NT * 4;
+  static constexpr int kFixedBytes = kBarrierBytes + kPartials * kScaleBytes;
+  static constexpr int kStages = (113 * 1024 - kFixedBytes) / kStageBytes;
+  static_assert(kStages >= 4 && kStages <= 8, "pipeline depth");
+  static_assert(NT * kBM * 4 <= kStages * kStageBytes, "the sums that CTAs exchange lie over the pipeline's stages");
+  static constexpr int kSmemBytes = kStages * kStageBytes + kFixedBytes;
+};
+
+__device__ __forceinline__ float finish_one(float y, const GemmFp8& g, int column) {
+  if (g.bias != nullptr) y += __bfloat162float(g.bias[column]);
+  if (g.activation == LC0B200_ACT_RELU) return y < 0.0f ? 0.0f : y;  // NaN stays
+  return activate_rt(y, g.activation);
+}
+
+__device__ __forceinline__ void store_one(float y, const GemmFp8& g, long long at) {
+  if (g.out_kind == LC0B200_OUT_F32) reinterpret_cast<float*>(g.out)[at] = y;
+  else reinterpret_cast<bf16*>(g.out)[at] = __float2bfloat16_rn(y);
+}
+
+template <int NT>
+__global__ void __launch_bounds__(Few<NT>::kThreads)
+gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const FpParams p) {
+  using T = Few<NT>;
+  constexpr int kStages = T::kStages;
+  constexpr int kPartials = T::kPartials;
+
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t smem_base = ptx::smem_u32(smem_raw);
+  const uint32_t smem_w = smem_base;
+  const uint32_t smem_a = smem_base + kStages * T::kWBytes;
+  const uint32_t bar_base = smem_base + kStages * T::kStageBytes;
+  const uint32_t bar_full = bar_base;                               // [kStages]
+  const uint32_t bar_empty = bar_base + 8 * kStages;                // [kStages]
+  const uint32_t bar_part_full = bar_base + 16 * kStages;           // [kPartials] product and scales are there
+  const uint32_t bar_part_empty = bar_part_full + 8 * kPartials;    // [kPartials]
+  const uint32_t tmem_slot = bar_part_empty + 8 * kPartials;
+  const uint32_t scale_base = bar_base + T::kBarrierBytes;          // [kPartials][NT] f32
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem_raw + (tmem_slot + 4 - smem_base));
+  static_assert(16 * kStages + 16 * kPartials + 8 <= T::kBarrierBytes, "barrier area too small");
+  grid_dependency_release();
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(ptx::cluster_ctarank());
+  const int splits = static_cast<int>(ptx::cluster_nctaid());
+  const GemmFp8& g = p.g;
+  const int n0 = static_cast<int>(blockIdx.x / splits) * kBM;
+  const int k_blocks = (g.k + kFp8Block - 1) / kFp8Block;
+  const int kb_begin = static_cast<int>(static_cast<long long>(k_blocks) * rank / splits);
+  const int kb_end = static_cast<int>(static_cast<long long>(k_blocks) * (rank + 1) / splits);
+  const bool aligned = (smem_base & 1023u) == 0u;  // never false; then nothing is computed rather than mis-swizzled
+  if (!aligned && threadIdx.x == 0 && atomicCAS(&p.status[0], 0u, kDeviceSmemMisaligned) == 0u) p.status[1] = smem_base;
+
+  if (threadIdx.x == 0) {
+    *abort_flag = aligned ? 0 : 1;
+    for (int s = 0; s < kStages; ++s) {
+      ptx::mbar_init(bar_full + 8 * s, 1);
+      ptx::mbar_init(bar_empty + 8 * s, 1);
+    }
+    for (int a = 0; a < kPartials; ++a) {
+      ptx::mbar_init(bar_part_full + 8 * a, 2);   // the MMAs' completion and a scale warp
+      ptx::mbar_init(bar_part_empty + 8 * a, 4);  // the epilogue warps
+    }
+    ptx::mbar_init_fence();
+    ptx::prefetch_tensormap(&map_w);
+    ptx::prefetch_tensormap(&map_a);
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc(tmem_slot, T::kTmemCols);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  ptx::tc_fence_after_sync();
+  uint32_t tmem_base;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem_base) : "r"(tmem_slot));
+  grid_dependency_wait();
+
+  bool ok = aligned;
+  if (warp == 0) {
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int kb = kb_begin; kb < kb_end && ok; ++kb) {
+      ok = ptx::mbar_wait(bar_empty + 8 * stage, phase ^ 1u, abort_flag, p.status, 0x2100u + stage);
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      if (!ok) break;
+      if (ptx::elect_one()) {
+        ptx::mbar_expect_tx(bar_full + 8 * stage, T::kStageBytes);
+        ptx::tma_load_2d<1>(smem_w + stage * T::kWBytes, &map_w, kb * kFp8Block, n0, bar_full + 8 * stage);
+        ptx::tma_load_2d<1>(smem_a + stage * NT * kRowBytes, &map_a, kb * kFp8Block, 0, bar_full + 8 * stage);
+      }
+      if (++stage == kStages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    constexpr uint32_t idesc = ptx::instr_desc(1u, 0u, 0u, kBM, NT);
+    int stage = 0, part = 0;
+    uint32_t phase = 0, part_phase = 0;
+    for (int kb = kb_begin; kb < kb_end && ok; ++kb) {
+      ok = ptx::mbar_wait(bar_part_empty + 8 * part, part_phase ^ 1u, abort_flag, p.status, 0x2200u + part);
+      ok = ok && ptx::mbar_wait(bar_full + 8 * stage, phase, abort_flag, p.status, 0x2300u + stage);
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      if (!ok) break;
+      ptx::tc_fence_after_sync();
+      if (ptx::elect_one()) {
+#pragma unroll
+        for (int j = 0; j < kFp8Block / kMmaK; ++j) {
+          mma_e4m3<1>(tmem_base + part * NT, ptx::smem_desc_sw128(smem_w + stage * T::kWBytes + j * kMmaK, 16, 1024),
+                      ptx::smem_desc_sw128(smem_a + stage * NT * kRowBytes + j * kMmaK, 16, 1024), idesc, j > 0 ? 1u : 0u);
+        }
+        ptx::tc_commit<1>(bar_empty + 8 * stage);
+        ptx::tc_commit<1>(bar_part_full + 8 * part);
+      }
+      if (++stage == kStages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+      if (++part == kPartials) {
+        part = 0;
+        part_phase ^= 1u;
+      }
+    }
+    __syncwarp();
+  } else if (warp < 4) {
+    // Scales: two warps take the k blocks in turn; lane j holds the products of tokens j and j + 32.
+    const float* w_scale = g.w_scale + (n0 / kFp8Block) * g.ld_w_scale;
+    const int first = warp - 2;
+    int part = first;
+    uint32_t phase = 0;
+    for (int kb = kb_begin + first; kb < kb_end && ok; kb += 2) {
+      const float w = __ldg(w_scale + kb);
+      const float a0 = lane < g.m ? __ldg(g.a_scale + kb * g.ld_a_scale + lane) : 0.0f;
+      const float a1 = NT > 32 && lane + 32 < g.m ? __ldg(g.a_scale + kb * g.ld_a_scale + lane + 32) : 0.0f;
+      ok = ptx::mbar_wait(bar_part_empty + 8 * part, phase ^ 1u, abort_flag, p.status, 0x2500u + part);
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      if (!ok) break;
+      const uint32_t dst = scale_base + part * T::kScaleBytes + lane * 4;
+      if (lane < NT) asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst), "f"(a0 * w) : "memory");
+      if (NT > 32) asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst + 128), "f"(a1 * w) : "memory");
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(bar_part_full + 8 * part);
+      part += 2;
+      if (part >= kPartials) {
+        part = first;
+        phase ^= 1u;
+      }
+    }
+    __syncwarp();
+  }
+  const int quarter = warp & 3;
+  const int row = quarter * 32 + lane;  // of the weight tile
+  float acc[NT];
+  if (warp >= 4) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[j] = 0.0f;
+    int part = 0;
+    uint32_t part_phase = 0;
+    for (int kb = kb_begin; kb < kb_end && ok; ++kb) {
+      ok = ptx::mbar_wait(bar_part_full + 8 * part, part_phase, abort_flag, p.status, 0x2400u + part);
+      if (!ok) break;
+      ptx::tc_fence_after_sync();
+      const uint32_t taddr = tmem_base + part * NT + (static_cast<uint32_t>(quarter * 32) << 16);
+      uint32_t v[NT];
+      tmem_ld_columns(taddr, v);
+      float s[NT];
+#pragma unroll
+      for (int j = 0; j < NT / 4; ++j) {
+        uint4 raw;
+        ptx::ld_shared_v4(scale_base + part * T::kScaleBytes + 16 * j, raw);
+        s[4 * j] = __uint_as_float(raw.x); s[4 * j + 1] = __uint_as_float(raw.y);
+        s[4 * j + 2] = __uint_as_float(raw.z); s[4 * j + 3] = __uint_as_float(raw.w);
+      }
+      tmem_wait(v);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) acc[j] = fmaf(__uint_as_float(v[j]), s[j], acc[j]);
+      ptx::tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(bar_part_empty + 8 * part);
+      if (++part == kPartials) {
+        part = 0;
+        part_phase ^= 1u;
+      }
+    }
+  }
+  const int column = n0 + row;
+  if (splits == 1) {
+    if (warp >= 4 && ok && column < g.n) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        if (j < g.m) store_one(finish_one(acc[j], g, column), g, j * g.ldc + column);
+      }
+    }
+  } else {
+    // Every product of this CTA has been formed and read: the stages are free for the exchange.  [token][weight row].
+    if (warp >= 4) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(smem_base + (j * kBM + row) * 4), "f"(acc[j]) : "memory");
+      }
+    }
+    __syncwarp();
+    ptx::cluster_sync();
+    // This CTA's share of the tokens, summed over the CTAs in their order.
+    if (warp >= 4 && ok && column < g.n) {
+      const int tokens = static_cast<int>(g.m);
+      for (int j = tokens * rank / splits; j < tokens * (rank + 1) / splits; ++j) {
+        float sum = 0.0f;
+        for (int r = 0; r < splits; ++r) {
+          float part;
+          asm volatile("ld.shared::cluster.f32 %0, [%1];"
+                       : "=f"(part)
+                       : "r"(ptx::map_to_cta(smem_base + (j * kBM + row) * 4, static_cast<uint32_t>(r)))
+                       : "memory");
+          sum += part;
+        }
+        store_one(finish_one(sum, g, column), g, j * g.ldc + column);
+      }
+    }
+    __syncwarp();
+    ptx::cluster_sync();  // nobody leaves while its sums may still be read
+  }
+
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    ptx::tc_fence_after_sync();
+    ptx::tmem_dealloc(tmem_base, T::kTmemCols);
+  }
+}
+
 bool make_map(CUtensorMap* map, const void* base, int elem_bytes, long long rows, long long cols, long long pitch,
               int box_rows, int box_cols) {
   return make_tensormap_2d(map, base, elem_bytes, rows, cols, pitch, box_rows, box_cols, CU_TENSOR_MAP_SWIZZLE_128B);
@@ -552,6 +825,45 @@ int launch(const GemmFp8& g, cudaStream_t stream) {
   return LC0B200_OK;
 }
 
+template <int NT>
+int launch_few(const GemmFp8& g, cudaStream_t stream) {
+  using T = Few<NT>;
+  CUtensorMap map_a, map_w;
+  if (!make_map(&map_w, g.w, 1, g.n, g.k, g.ldw, kBM, kFp8Block)) return LC0B200_ERR_CUDA;
+  if (!make_map(&map_a, g.a, 1, g.m, g.k, g.lda, NT, kFp8Block)) return LC0B200_ERR_CUDA;
+  FpParams p;
+  p.g = g;
+  p.tma_store = 0;
+  p.status = device_status_words();
+  if (p.status == nullptr) return LC0B200_ERR_CUDA;
+  auto kernel = gemm_fp8_few_kernel<NT>;
+  static PerDeviceOnce smem_opt_in;  // per instantiation
+  if (allow_dynamic_smem(smem_opt_in, kernel, T::kSmemBytes) != LC0B200_OK) return LC0B200_ERR_CUDA;
+  // Split k while that keeps the grid within one CTA per SM (clusters of at most 8, a k block each at least).
+  const long long tiles = ceil_div_ll(g.n, kBM);
+  const int k_blocks = static_cast<int>(ceil_div_ll(g.k, kFp8Block));
+  int splits = 1;
+  while (splits < 8 && 2 * splits <= k_blocks && tiles * splits * 2 <= sm_count()) splits *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * splits));
+  cfg.blockDim = dim3(T::kThreads);
+  cfg.dynamicSmemBytes = T::kSmemBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0] = dependent_launch_attribute();
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = splits;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = splits > 1 ? 2 : 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, map_w, map_a, p) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return LC0B200_ERR_CUDA;
+  }
+  return LC0B200_OK;
+}
+
 }  // namespace
 
 int gemm_fp8(const GemmFp8& given, cudaStream_t stream) {
@@ -560,6 +872,9 @@ int gemm_fp8(const GemmFp8& given, cudaStream_t stream) {
   if (g.m == 1) g.lda = ceil_div_ll(g.k, 16) * 16;
   if (g.n == 1) g.ldw = ceil_div_ll(g.k, 16) * 16;
   if (!aligned16(g.a) || !aligned16(g.w) || (g.lda % 16) != 0 || (g.ldw % 16) != 0) return gemm_fp8_simt(g, stream);
+  if (g.m <= 16) return launch_few<16>(g, stream);
+  if (g.m <= 32) return launch_few<32>(g, stream);
+  if (g.m <= 64) return launch_few<64>(g, stream);
   // The widest tile that still gives most SMs one.
   const long long enough = sm_count() * 3LL / 5;
   if (2 * ceil_div_ll(g.m, 2 * kBM) * ceil_div_ll(g.n, 256) >= enough) return launch<256, 2>(g, stream);

@@ -246,35 +246,54 @@ def linear_int8_static(out: torch.Tensor, a: torch.Tensor, w_nk: torch.Tensor, c
 # ---- 8-bit floating point (e4m3, blocks of 128).  These wrappers take shapes and pitches from 2-D tensors.
 
 FP8_BLOCK = 128
+_FP8_OUT_KIND = {torch.bfloat16: _lib.OUT_BF16, torch.float32: _lib.OUT_F32}
 
 
-def _matrix(t: torch.Tensor, dtype: torch.dtype, name: str, rows: int, columns: int) -> int:
-    """Check a 2-D tensor on the current device whose rows are contiguous; return its row pitch."""
-    _require(t, dtype, name)
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != columns:
-        raise ValueError(f"{name} must have shape [{rows}, {columns}], got {list(t.shape)}")
-    if t.device.index != torch.cuda.current_device():
+def _raw_stream(device: int) -> int:
+    # torch.cuda.current_stream() builds a Stream object: 3 us of a call whose kernel may take 2.
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
+def _device_of(t: torch.Tensor, name: str) -> int:
+    """The device a call works on: the first operand's, which has to be the current one."""
+    device = t.get_device()
+    if device < 0:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if device != torch.cuda.current_device():
         raise ValueError(f"{name} is on {t.device}, not on the current CUDA device")
+    return device
+
+
+def _refuse(t: torch.Tensor, dtype: torch.dtype, name: str, shape: tuple[int, ...], device: int) -> None:
+    _require(t, dtype, name)
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must have shape {list(shape)}, got {list(t.shape)}")
+    raise ValueError(f"{name} is on {t.device}, not on cuda:{device}")
+
+
+def _matrix(t: torch.Tensor, dtype: torch.dtype, name: str, rows: int, columns: int, device: int) -> int:
+    """Check a 2-D tensor on the call's device whose rows are contiguous; return its row pitch."""
+    if t.dtype is not dtype or t.shape != (rows, columns) or t.get_device() != device:
+        _refuse(t, dtype, name, (rows, columns), device)
     row, column = t.stride()
     if column != 1 and columns > 1:
         raise ValueError(f"{name} must have contiguous rows")
-    return row if rows > 1 else max(row, columns)  # the stride of a single row says nothing
+    return row if rows > 1 or row > columns else columns  # the stride of a single row says nothing
 
 
-def _vector(t: torch.Tensor, name: str, size: int) -> None:
-    _require(t, torch.bfloat16, name)
-    if t.dim() != 1 or t.shape[0] != size or (size > 1 and t.stride(0) != 1):
-        raise ValueError(f"{name} must be a contiguous vector of {size} elements")
-    if t.device.index != torch.cuda.current_device():
-        raise ValueError(f"{name} is on {t.device}, not on the current CUDA device")
+def _vector(t: torch.Tensor, name: str, size: int, device: int) -> None:
+    if t.dtype is not torch.bfloat16 or t.shape != (size,) or t.get_device() != device:
+        _refuse(t, torch.bfloat16, name, (size,), device)
+    if size > 1 and t.stride(0) != 1:
+        raise ValueError(f"{name} must be contiguous")
 
 
-def _scratch(t: torch.Tensor, name: str, dtype: torch.dtype, size: int) -> None:
+def _scratch(t: torch.Tensor, name: str, dtype: torch.dtype, size: int, device: int) -> None:
     _require(t, dtype, name)
     if not t.is_contiguous() or t.numel() < size:
         raise ValueError(f"{name} must be contiguous and hold at least {size} elements")
-    if t.device.index != torch.cuda.current_device():
-        raise ValueError(f"{name} is on {t.device}, not on the current CUDA device")
+    if t.get_device() != device:
+        raise ValueError(f"{name} is on {t.device}, not on cuda:{device}")
 
 
 def quantize_fp8(out: torch.Tensor, scale: torch.Tensor, x: torch.Tensor, *,
@@ -284,16 +303,17 @@ def quantize_fp8(out: torch.Tensor, scale: torch.Tensor, x: torch.Tensor, *,
     ``block_rows=128``: weights, ``scale [ceil(rows/128), ceil(width/128)]``."""
     if block_rows not in (1, FP8_BLOCK):
         raise ValueError("block_rows must be 1 or 128")
+    device = _device_of(x, "x")
     rows, width = x.shape
     blocks = -(-width // FP8_BLOCK)
-    ld_in = _matrix(x, torch.bfloat16, "x", rows, width)
-    ld_out = _matrix(out, torch.float8_e4m3fn, "out", rows, width)
-    ld_scale = (_matrix(scale, torch.float32, "scale", blocks, rows) if block_rows == 1 else
-                _matrix(scale, torch.float32, "scale", -(-rows // FP8_BLOCK), blocks))
+    ld_in = _matrix(x, torch.bfloat16, "x", rows, width, device)
+    ld_out = _matrix(out, torch.float8_e4m3fn, "out", rows, width, device)
+    ld_scale = (_matrix(scale, torch.float32, "scale", blocks, rows, device) if block_rows == 1 else
+                _matrix(scale, torch.float32, "scale", -(-rows // FP8_BLOCK), blocks, device))
     if rows == 0:  # an empty tensor has no address
         return out, scale
     check(_lib.load().lc0b200_quantize_fp8(_p(out), _p(scale), _p(x), rows, width, block_rows, ld_in, ld_out, ld_scale,
-                                           _stream()), "quantize_fp8")
+                                           _raw_stream(device)), "quantize_fp8")
     return out, scale
 
 
@@ -305,31 +325,33 @@ def rms_norm(out: torch.Tensor | None, x: torch.Tensor, gammas: torch.Tensor, *,
     ``residual_out`` receives ``v`` (needs ``skip``; may be ``x`` or ``skip`` itself, as may ``out``); ``q_out`` /
     ``q_scale [ceil(width/128), rows]`` the result as e4m3 codes with a scale per 128 values.  ``out`` may be None
     when the codes are asked for."""
+    device = _device_of(x, "x")
     rows, width = x.shape
     bf = torch.bfloat16
-    ld_in = _matrix(x, bf, "x", rows, width)
-    _vector(gammas, "gammas", width)
-    ld_skip = 0 if skip is None else _matrix(skip, bf, "skip", rows, width)
-    ld_out = 0 if out is None else _matrix(out, bf, "out", rows, width)
-    ld_residual = 0 if residual_out is None else _matrix(residual_out, bf, "residual_out", rows, width)
+    ld_in = _matrix(x, bf, "x", rows, width, device)
+    _vector(gammas, "gammas", width, device)
+    ld_skip = 0 if skip is None else _matrix(skip, bf, "skip", rows, width, device)
+    ld_out = 0 if out is None else _matrix(out, bf, "out", rows, width, device)
+    ld_residual = 0 if residual_out is None else _matrix(residual_out, bf, "residual_out", rows, width, device)
     ld_q = ld_scale = 0
     if q_out is not None and q_scale is not None:
-        ld_q = _matrix(q_out, torch.float8_e4m3fn, "q_out", rows, width)
-        ld_scale = _matrix(q_scale, torch.float32, "q_scale", -(-width // FP8_BLOCK), rows)
+        ld_q = _matrix(q_out, torch.float8_e4m3fn, "q_out", rows, width, device)
+        ld_scale = _matrix(q_scale, torch.float32, "q_scale", -(-width // FP8_BLOCK), rows, device)
     if rows == 0:
         return out
     check(_lib.load().lc0b200_rms_norm(_p(out), _p(residual_out), _p(q_out), _p(q_scale), _p(x), _p(skip), _p(gammas),
                                        rows, width, epsilon, ld_in, ld_skip, ld_out, ld_residual, ld_q, ld_scale,
-                                       _stream()), "rms_norm")
+                                       _raw_stream(device)), "rms_norm")
     return out
 
 
-def _fp8_weight(w: torch.Tensor, w_scale: torch.Tensor, bias: torch.Tensor | None, k: int) -> tuple[int, int, int]:
+def _fp8_weight(w: torch.Tensor, w_scale: torch.Tensor, bias: torch.Tensor | None, k: int,
+                device: int) -> tuple[int, int, int]:
     n = w.shape[0]
     if bias is not None:
-        _vector(bias, "bias", n)
-    return (n, _matrix(w, torch.float8_e4m3fn, "w", n, k),
-            _matrix(w_scale, torch.float32, "w_scale", -(-n // FP8_BLOCK), -(-k // FP8_BLOCK)))
+        _vector(bias, "bias", n, device)
+    return (n, _matrix(w, torch.float8_e4m3fn, "w", n, k, device),
+            _matrix(w_scale, torch.float32, "w_scale", -(-n // FP8_BLOCK), -(-k // FP8_BLOCK), device))
 
 
 def gemm_fp8(out: torch.Tensor, a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *,
@@ -338,17 +360,19 @@ def gemm_fp8(out: torch.Tensor, a: torch.Tensor, a_scale: torch.Tensor, w: torch
     (``include/lc0b200.h``: lc0b200_gemm_fp8): ``a_scale [ceil(k/128), m]``, ``w_scale [ceil(n/128), ceil(k/128)]``.
     ``out`` is bf16 or f32.  Keep row pitches and bases of ``a`` and ``w`` at multiples of 16 bytes: others run on
     the CUDA cores."""
+    device = _device_of(a, "a")
     m, k = a.shape
-    lda = _matrix(a, torch.float8_e4m3fn, "a", m, k)
-    ld_a_scale = _matrix(a_scale, torch.float32, "a_scale", -(-k // FP8_BLOCK), m)
-    n, ldw, ld_w_scale = _fp8_weight(w, w_scale, bias, k)
-    if out.dtype not in (torch.bfloat16, torch.float32):
+    lda = _matrix(a, torch.float8_e4m3fn, "a", m, k, device)
+    ld_a_scale = _matrix(a_scale, torch.float32, "a_scale", -(-k // FP8_BLOCK), m, device)
+    n, ldw, ld_w_scale = _fp8_weight(w, w_scale, bias, k, device)
+    kind = _FP8_OUT_KIND.get(out.dtype)
+    if kind is None:
         raise ValueError(f"out must be bfloat16 or float32, got {out.dtype}")
-    ldc = _matrix(out, out.dtype, "out", m, n)
+    ldc = _matrix(out, out.dtype, "out", m, n, device)
     if m == 0:
         return out
     check(_lib.load().lc0b200_gemm_fp8(_p(out), _p(a), _p(a_scale), _p(w), _p(w_scale), _p(bias), m, n, k, lda, ld_a_scale,
-                                       ldw, ld_w_scale, ldc, _OUT_KIND[out.dtype], ACTIVATIONS[activation], _stream()),
+                                       ldw, ld_w_scale, ldc, kind, ACTIVATIONS[activation], _raw_stream(device)),
           "gemm_fp8")
     return out
 
@@ -357,19 +381,21 @@ def linear_fp8(out: torch.Tensor, a: torch.Tensor, w: torch.Tensor, w_scale: tor
                scratch_q: torch.Tensor, scratch_scale: torch.Tensor, *, activation: str = "none") -> torch.Tensor:
     """bf16 activations -> e4m3 codes and scales (into caller scratch) -> ``gemm_fp8``.  ``scratch_q`` is any contiguous
     tensor of at least ``m * (k rounded up to 16)`` bytes, ``scratch_scale`` of at least ``m * ceil(k/128)`` floats."""
+    device = _device_of(a, "a")
     m, k = a.shape
-    lda = _matrix(a, torch.bfloat16, "a", m, k)
-    n, ldw, ld_w_scale = _fp8_weight(w, w_scale, bias, k)
-    if out.dtype not in (torch.bfloat16, torch.float32):
+    lda = _matrix(a, torch.bfloat16, "a", m, k, device)
+    n, ldw, ld_w_scale = _fp8_weight(w, w_scale, bias, k, device)
+    kind = _FP8_OUT_KIND.get(out.dtype)
+    if kind is None:
         raise ValueError(f"out must be bfloat16 or float32, got {out.dtype}")
-    ldc = _matrix(out, out.dtype, "out", m, n)
-    _scratch(scratch_q, "scratch_q", torch.float8_e4m3fn, m * -(-k // 16) * 16)
-    _scratch(scratch_scale, "scratch_scale", torch.float32, m * -(-k // FP8_BLOCK))
+    ldc = _matrix(out, out.dtype, "out", m, n, device)
+    _scratch(scratch_q, "scratch_q", torch.float8_e4m3fn, m * -(-k // 16) * 16, device)
+    _scratch(scratch_scale, "scratch_scale", torch.float32, m * -(-k // FP8_BLOCK), device)
     if m == 0:
         return out
     check(_lib.load().lc0b200_linear_fp8(_p(out), _p(a), _p(w), _p(w_scale), _p(bias), _p(scratch_q), _p(scratch_scale),
-                                         m, n, k, lda, ldw, ld_w_scale, ldc, _OUT_KIND[out.dtype],
-                                         ACTIVATIONS[activation], _stream()), "linear_fp8", launches=2)
+                                         m, n, k, lda, ldw, ld_w_scale, ldc, kind,
+                                         ACTIVATIONS[activation], _raw_stream(device)), "linear_fp8", launches=2)
     return out
 
 
