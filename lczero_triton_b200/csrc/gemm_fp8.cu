@@ -7,7 +7,7 @@
 //
 // gemm_fp8_kernel (many rows): persistent, tiles of 128 x BN per CTA, or 256 x 256 per CTA pair (cta_group::2; each CTA
 // loads its own rows of A and its own half of W with plain TMA loads, none is multicast).  Warp 0 loads (one elected
-// lane), warp 1 issues the MMAs, warps 4 and up are the epilogue: two per TMEM lane quarter for BN >= 128, each with half
+// lane), warp 1 issues the MMAs, warps 4 and up are the epilogue: two per TMEM lane quarter, each with half
 // of the columns.
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -68,11 +68,7 @@ __device__ __forceinline__ void tmem_wait(uint32_t (&v)[16]) {
                :
                : "memory");
 }
-__device__ __forceinline__ void tmem_wait(uint32_t (&v)[64]) {
-  tmem_wait(*reinterpret_cast<uint32_t(*)[32]>(&v[0]));
-  tmem_wait(*reinterpret_cast<uint32_t(*)[32]>(&v[32]));
-}
-// 32 lanes x 16 / 32 / 64 columns of tensor memory.
+// 32 lanes x 16 or 32 columns of tensor memory.
 __device__ __forceinline__ void tmem_ld_columns(uint32_t taddr, uint32_t (&v)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
@@ -83,7 +79,6 @@ __device__ __forceinline__ void tmem_ld_columns(uint32_t taddr, uint32_t (&v)[16
       : "memory");
 }
 __device__ __forceinline__ void tmem_ld_columns(uint32_t taddr, uint32_t (&v)[32]) { ptx::tmem_ld_32x32(taddr, v); }
-__device__ __forceinline__ void tmem_ld_columns(uint32_t taddr, uint32_t (&v)[64]) { ptx::tmem_ld_32x64(taddr, v); }
 
 // A look at a barrier that never suspends.
 __device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity) {
@@ -130,10 +125,10 @@ struct Tile {
   // Block products in flight in tensor memory.  (A 256-wide tile as two half products with barriers of their own, so that
   // one is handed on while the other is multiplied, was measured slower: 163 us against 139 at 32768 x 1024 x 4096.
   // MMAs 128 wide are limited by their operand reads from shared memory.)
-  static constexpr int kPartials = BN == 256 ? 2 : 4;
-  static constexpr int kTmemCols = kPartials * BN;  // 512, 512, 256: powers of two
-  static constexpr int kEpilogueWarps = BN >= 128 ? 8 : 4;
-  static constexpr int kCols = BN / (kEpilogueWarps / 4);  // columns per epilogue thread: 128, 64, 64
+  static constexpr int kPartials = 512 / BN;
+  static constexpr int kTmemCols = kPartials * BN;
+  static constexpr int kEpilogueWarps = 8;
+  static constexpr int kCols = BN / (kEpilogueWarps / 4);  // columns per epilogue thread: 128 or 64
   // Four warps in front of the epilogue: loads, MMAs, and two that fetch the scales.
   static constexpr int kThreads = 128 + 32 * kEpilogueWarps;
   // 128 running sums a thread do not fit into an even share of the registers (65536 / 384 threads = 168): the first
@@ -526,18 +521,21 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
 
 // ---------------------------------------------------------------- few rows
 //
-// At most 64 rows of A: the weight's bytes are the work, and a 128-row tile of A would be mostly padding.  So the roles
-// are turned round: 128 weight rows are the M side of the MMA, the tokens its N side (NT = 16, 32 or 64 columns), and
-// out^T comes out: an epilogue thread owns one weight row, a block's scales are one product per token.  The k blocks of a
-// tile are split over the CTAs of a cluster, so that a layer of a few tiles still pulls on the memory of most SMs; their
-// sums meet in distributed shared memory, added in the order of the CTAs (the same bits every time).  Half of an SM's
-// shared memory per CTA, so that the next tile's loads can start while a CTA finishes.
+// Too few rows of A for 128-row tiles to fill the SMs: the weight's bytes are the work, and a 128-row tile of A would be
+// mostly padding.  So the roles are turned round: 128 weight rows are the M side of the MMA, NT = 16, 32 or 64 tokens its
+// N side, and out^T comes out: an epilogue thread owns one weight row, a block's scales are one product per token.  The k
+// blocks of a tile are split over the CTAs of a cluster, so that a layer of a few tiles still pulls on the memory of every
+// SM; their sums meet in distributed shared memory, added in the order of the CTAs (the same bits every time).  A CTA
+// takes half of an SM's shared memory and registers: two are resident, one loads while the other finishes.
+constexpr int kMaxSplits = 8;  // CTAs of a cluster (the portable limit)
+
 template <int NT>
 struct Few {
   static constexpr int kWBytes = kBM * kRowBytes;
   static constexpr int kStageBytes = kWBytes + NT * kRowBytes;
   static constexpr int kPartials = 4;
   static constexpr int kTmemCols = kPartials * NT;  // 64, 128, 256
+  static constexpr int kChunk = NT < 32 ? NT : 32;  // columns read back at a time
   static constexpr int kThreads = 256;              // warps: loads, MMAs, two for scales, four epilogue
   static constexpr int kBarrierBytes = 512;
   static constexpr int kScaleBytes = NT * 4;
@@ -560,7 +558,7 @@ __device__ __forceinline__ void store_one(float y, const GemmFp8& g, long long a
 }
 
 template <int NT>
-__global__ void __launch_bounds__(Few<NT>::kThreads)
+__global__ void __launch_bounds__(Few<NT>::kThreads, 2)
 gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const FpParams p) {
   using T = Few<NT>;
   constexpr int kStages = T::kStages;
@@ -586,7 +584,12 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
   const int rank = static_cast<int>(ptx::cluster_ctarank());
   const int splits = static_cast<int>(ptx::cluster_nctaid());
   const GemmFp8& g = p.g;
-  const int n0 = static_cast<int>(blockIdx.x / splits) * kBM;
+  // Token tiles of one weight tile are neighbours: they share its bytes in the L2.
+  const int token_tiles = static_cast<int>((g.m + NT - 1) / NT);
+  const int tile = static_cast<int>(blockIdx.x) / splits;
+  const int n0 = tile / token_tiles * kBM;
+  const long long m0 = static_cast<long long>(tile % token_tiles) * NT;
+  const int tokens = static_cast<int>(min(static_cast<long long>(NT), g.m - m0));
   const int k_blocks = (g.k + kFp8Block - 1) / kFp8Block;
   const int kb_begin = static_cast<int>(static_cast<long long>(k_blocks) * rank / splits);
   const int kb_end = static_cast<int>(static_cast<long long>(k_blocks) * (rank + 1) / splits);
@@ -629,7 +632,8 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
       if (ptx::elect_one()) {
         ptx::mbar_expect_tx(bar_full + 8 * stage, T::kStageBytes);
         ptx::tma_load_2d<1>(smem_w + stage * T::kWBytes, &map_w, kb * kFp8Block, n0, bar_full + 8 * stage);
-        ptx::tma_load_2d<1>(smem_a + stage * NT * kRowBytes, &map_a, kb * kFp8Block, 0, bar_full + 8 * stage);
+        ptx::tma_load_2d<1>(smem_a + stage * NT * kRowBytes, &map_a, kb * kFp8Block, static_cast<int>(m0),
+                            bar_full + 8 * stage);
       }
       if (++stage == kStages) {
         stage = 0;
@@ -674,8 +678,9 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     uint32_t phase = 0;
     for (int kb = kb_begin + first; kb < kb_end && ok; kb += 2) {
       const float w = __ldg(w_scale + kb);
-      const float a0 = lane < g.m ? __ldg(g.a_scale + kb * g.ld_a_scale + lane) : 0.0f;
-      const float a1 = NT > 32 && lane + 32 < g.m ? __ldg(g.a_scale + kb * g.ld_a_scale + lane + 32) : 0.0f;
+      const float* a_scale = g.a_scale + kb * g.ld_a_scale + m0;
+      const float a0 = lane < tokens ? __ldg(a_scale + lane) : 0.0f;
+      const float a1 = NT > 32 && lane + 32 < tokens ? __ldg(a_scale + lane + 32) : 0.0f;
       ok = ptx::mbar_wait(bar_part_empty + 8 * part, phase ^ 1u, abort_flag, p.status, 0x2500u + part);
       ok = __all_sync(0xFFFFFFFFu, ok);
       if (!ok) break;
@@ -705,19 +710,22 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
       if (!ok) break;
       ptx::tc_fence_after_sync();
       const uint32_t taddr = tmem_base + part * NT + (static_cast<uint32_t>(quarter * 32) << 16);
-      uint32_t v[NT];
-      tmem_ld_columns(taddr, v);
-      float s[NT];
 #pragma unroll
-      for (int j = 0; j < NT / 4; ++j) {
-        uint4 raw;
-        ptx::ld_shared_v4(scale_base + part * T::kScaleBytes + 16 * j, raw);
-        s[4 * j] = __uint_as_float(raw.x); s[4 * j + 1] = __uint_as_float(raw.y);
-        s[4 * j + 2] = __uint_as_float(raw.z); s[4 * j + 3] = __uint_as_float(raw.w);
+      for (int c = 0; c < NT; c += T::kChunk) {
+        uint32_t v[T::kChunk];
+        tmem_ld_columns(taddr + c, v);
+        float s[T::kChunk];
+#pragma unroll
+        for (int j = 0; j < T::kChunk / 4; ++j) {
+          uint4 raw;
+          ptx::ld_shared_v4(scale_base + part * T::kScaleBytes + (c + 4 * j) * 4, raw);
+          s[4 * j] = __uint_as_float(raw.x); s[4 * j + 1] = __uint_as_float(raw.y);
+          s[4 * j + 2] = __uint_as_float(raw.z); s[4 * j + 3] = __uint_as_float(raw.w);
+        }
+        tmem_wait(v);
+#pragma unroll
+        for (int j = 0; j < T::kChunk; ++j) acc[c + j] = fmaf(__uint_as_float(v[j]), s[j], acc[c + j]);
       }
-      tmem_wait(v);
-#pragma unroll
-      for (int j = 0; j < NT; ++j) acc[j] = fmaf(__uint_as_float(v[j]), s[j], acc[j]);
       ptx::tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(bar_part_empty + 8 * part);
@@ -727,43 +735,55 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
       }
     }
   }
-  const int column = n0 + row;
-  if (splits == 1) {
-    if (warp >= 4 && ok && column < g.n) {
+  // Every product of this CTA has been formed and read: the stages are free for the exchange.  [token][weight row].
+  if (warp >= 4) {
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        if (j < g.m) store_one(finish_one(acc[j], g, column), g, j * g.ldc + column);
-      }
+    for (int j = 0; j < NT; ++j) {
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(smem_base + (j * kBM + row) * 4), "f"(acc[j]) : "memory");
     }
-  } else {
-    // Every product of this CTA has been formed and read: the stages are free for the exchange.  [token][weight row].
-    if (warp >= 4) {
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        asm volatile("st.shared.f32 [%0], %1;" ::"r"(smem_base + (j * kBM + row) * 4), "f"(acc[j]) : "memory");
-      }
-    }
-    __syncwarp();
-    ptx::cluster_sync();
-    // This CTA's share of the tokens, summed over the CTAs in their order.
-    if (warp >= 4 && ok && column < g.n) {
-      const int tokens = static_cast<int>(g.m);
-      for (int j = tokens * rank / splits; j < tokens * (rank + 1) / splits; ++j) {
-        float sum = 0.0f;
-        for (int r = 0; r < splits; ++r) {
-          float part;
-          asm volatile("ld.shared::cluster.f32 %0, [%1];"
-                       : "=f"(part)
-                       : "r"(ptx::map_to_cta(smem_base + (j * kBM + row) * 4, static_cast<uint32_t>(r)))
-                       : "memory");
-          sum += part;
-        }
-        store_one(finish_one(sum, g, column), g, j * g.ldc + column);
-      }
-    }
-    __syncwarp();
-    ptx::cluster_sync();  // nobody leaves while its sums may still be read
   }
+  __syncwarp();
+  ptx::cluster_sync();
+  // This CTA's share of the tokens, summed over the CTAs in their order: a thread takes four neighbouring columns of
+  // a token, a warp a token at a time (every warp of the CTA), and asks for all CTAs' pieces before it adds them.
+  if (*abort_flag == 0) {
+    const int col0 = n0 + 4 * lane;
+    const bool four = col0 + 4 <= g.n && g.out_kind == LC0B200_OUT_BF16 && (g.ldc % 4) == 0 &&
+                      (reinterpret_cast<uintptr_t>(g.out) % 8) == 0;
+    for (int j = tokens * rank / splits + warp; j < tokens * (rank + 1) / splits; j += T::kThreads / 32) {
+      float piece[kMaxSplits][4];
+#pragma unroll
+      for (int r = 0; r < kMaxSplits; ++r) {
+        if (r < splits) {
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(piece[r][0]), "=f"(piece[r][1]), "=f"(piece[r][2]), "=f"(piece[r][3])
+                       : "r"(ptx::map_to_cta(smem_base + (j * kBM + 4 * lane) * 4, static_cast<uint32_t>(r)))
+                       : "memory");
+        }
+      }
+      float y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float sum = piece[0][i];
+#pragma unroll
+        for (int r = 1; r < kMaxSplits; ++r) {
+          if (r < splits) sum += piece[r][i];
+        }
+        y[i] = col0 + i < g.n ? finish_one(sum, g, col0 + i) : 0.0f;
+      }
+      const long long at = (m0 + j) * g.ldc + col0;
+      if (four) {
+        *reinterpret_cast<uint2*>(reinterpret_cast<bf16*>(g.out) + at) = make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (col0 + i < g.n) store_one(y[i], g, at + i);
+        }
+      }
+    }
+  }
+  __syncwarp();
+  ptx::cluster_sync();  // nobody leaves while its sums may still be read
 
   ptx::tc_fence_before_sync();
   __syncthreads();
@@ -839,11 +859,12 @@ int launch_few(const GemmFp8& g, cudaStream_t stream) {
   auto kernel = gemm_fp8_few_kernel<NT>;
   static PerDeviceOnce smem_opt_in;  // per instantiation
   if (allow_dynamic_smem(smem_opt_in, kernel, T::kSmemBytes) != LC0B200_OK) return LC0B200_ERR_CUDA;
-  // Split k while that keeps the grid within one CTA per SM (clusters of at most 8, a k block each at least).
-  const long long tiles = ceil_div_ll(g.n, kBM);
+  // Split k while every CTA stays resident, two to an SM, and has a k block at least.
+  const long long tiles = ceil_div_ll(g.n, kBM) * ceil_div_ll(g.m, NT);
+  if (tiles > 0x7FFFFFFFLL / kMaxSplits) return LC0B200_ERR_UNSUPPORTED;
   const int k_blocks = static_cast<int>(ceil_div_ll(g.k, kFp8Block));
   int splits = 1;
-  while (splits < 8 && 2 * splits <= k_blocks && tiles * splits * 2 <= sm_count()) splits *= 2;
+  while (splits < kMaxSplits && 2 * splits <= k_blocks && tiles * splits <= sm_count()) splits *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(tiles * splits));
   cfg.blockDim = dim3(T::kThreads);
@@ -879,7 +900,7 @@ int gemm_fp8(const GemmFp8& given, cudaStream_t stream) {
   const long long enough = sm_count() * 3LL / 5;
   if (2 * ceil_div_ll(g.m, 2 * kBM) * ceil_div_ll(g.n, 256) >= enough) return launch<256, 2>(g, stream);
   if (ceil_div_ll(g.m, kBM) * ceil_div_ll(g.n, 128) >= enough) return launch<128, 1>(g, stream);
-  return launch<64, 1>(g, stream);
+  return launch_few<64>(g, stream);
 }
 
 }  // namespace lc0b200
