@@ -525,8 +525,10 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
 // mostly padding.  So the roles are turned round: 128 weight rows are the M side of the MMA, NT = 16, 32 or 64 tokens its
 // N side, and out^T comes out: an epilogue thread owns one weight row, a block's scales are one product per token.  The k
 // blocks of a tile are split over the CTAs of a cluster, so that a layer of a few tiles still pulls on the memory of every
-// SM; their sums meet in distributed shared memory, added in the order of the CTAs (the same bits every time).  A CTA
-// takes half of an SM's shared memory and registers: two are resident, one loads while the other finishes.
+// SM.  Token j is finished by CTA j mod S: each CTA writes its sums for it straight into that CTA's shared memory, one
+// cluster barrier later the owner adds the S pieces in the order of the CTAs (the same bits every time) and stores.
+// (Fetching the pieces from the other CTAs instead took 2600 cycles a token and a second barrier of 2000.)  A CTA takes half
+// of an SM's shared memory and registers: two are resident, one loads while the other finishes.
 constexpr int kMaxSplits = 8;  // CTAs of a cluster (the portable limit)
 
 template <int NT>
@@ -535,14 +537,16 @@ struct Few {
   static constexpr int kStageBytes = kWBytes + NT * kRowBytes;
   static constexpr int kPartials = 4;
   static constexpr int kTmemCols = kPartials * NT;  // 64, 128, 256
-  static constexpr int kChunk = NT < 32 ? NT : 32;  // columns read back at a time
-  static constexpr int kThreads = 256;              // warps: loads, MMAs, two for scales, four epilogue
+  // Epilogue warps: four, or eight with half of the columns each.
+  static constexpr int kEpilogueWarps = NT == 64 ? 8 : 4;
+  static constexpr int kCols = NT / (kEpilogueWarps / 4);  // 16 or 32
+  static constexpr int kThreads = 128 + 32 * kEpilogueWarps;  // in front: loads, MMAs, two for scales
   static constexpr int kBarrierBytes = 512;
   static constexpr int kScaleBytes = NT * 4;
-  static constexpr int kFixedBytes = kBarrierBytes + kPartials * kScaleBytes;
+  static constexpr int kSumBytes = NT * kBM * 4;  // what the CTAs of a cluster write here: [CTA][token / S][weight row] f32
+  static constexpr int kFixedBytes = kSumBytes + kBarrierBytes + kPartials * kScaleBytes;
   static constexpr int kStages = (113 * 1024 - kFixedBytes) / kStageBytes;
-  static_assert(kStages >= 4 && kStages <= 8, "pipeline depth");
-  static_assert(NT * kBM * 4 <= kStages * kStageBytes, "the sums that CTAs exchange lie over the pipeline's stages");
+  static_assert(kStages >= 3 && kStages <= 8, "pipeline depth");
   static constexpr int kSmemBytes = kStages * kStageBytes + kFixedBytes;
 };
 
@@ -568,7 +572,8 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
   const uint32_t smem_base = ptx::smem_u32(smem_raw);
   const uint32_t smem_w = smem_base;
   const uint32_t smem_a = smem_base + kStages * T::kWBytes;
-  const uint32_t bar_base = smem_base + kStages * T::kStageBytes;
+  const uint32_t sums = smem_base + kStages * T::kStageBytes;
+  const uint32_t bar_base = sums + T::kSumBytes;
   const uint32_t bar_full = bar_base;                               // [kStages]
   const uint32_t bar_empty = bar_base + 8 * kStages;                // [kStages]
   const uint32_t bar_part_full = bar_base + 16 * kStages;           // [kPartials] product and scales are there
@@ -582,7 +587,8 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int rank = static_cast<int>(ptx::cluster_ctarank());
-  const int splits = static_cast<int>(ptx::cluster_nctaid());
+  const int split_bits = 31 - __clz(static_cast<int>(ptx::cluster_nctaid()));  // S is a power of two
+  const int splits = 1 << split_bits;
   const GemmFp8& g = p.g;
   // Token tiles of one weight tile are neighbours: they share its bytes in the L2.
   const int token_tiles = static_cast<int>((g.m + NT - 1) / NT);
@@ -604,7 +610,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     }
     for (int a = 0; a < kPartials; ++a) {
       ptx::mbar_init(bar_part_full + 8 * a, 2);   // the MMAs' completion and a scale warp
-      ptx::mbar_init(bar_part_empty + 8 * a, 4);  // the epilogue warps
+      ptx::mbar_init(bar_part_empty + 8 * a, T::kEpilogueWarps);
     }
     ptx::mbar_init_fence();
     ptx::prefetch_tensormap(&map_w);
@@ -616,6 +622,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
   }
   ptx::tc_fence_before_sync();
   __syncthreads();
+  ptx::cluster_arrive_relaxed();  // "this CTA runs": awaited before the first write into another CTA's memory
   ptx::tc_fence_after_sync();
   uint32_t tmem_base;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem_base) : "r"(tmem_slot));
@@ -699,33 +706,30 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
   }
   const int quarter = warp & 3;
   const int row = quarter * 32 + lane;  // of the weight tile
-  float acc[NT];
+  const int col = NT == 64 ? ((warp - 4) >> 2) * T::kCols : 0;  // this warp's first token
+  uint64_t acc[T::kCols / 2];  // running sums of two neighbouring tokens each
   if (warp >= 4) {
 #pragma unroll
-    for (int j = 0; j < NT; ++j) acc[j] = 0.0f;
+    for (int j = 0; j < T::kCols / 2; ++j) acc[j] = 0ull;
     int part = 0;
     uint32_t part_phase = 0;
     for (int kb = kb_begin; kb < kb_end && ok; ++kb) {
       ok = ptx::mbar_wait(bar_part_full + 8 * part, part_phase, abort_flag, p.status, 0x2400u + part);
       if (!ok) break;
       ptx::tc_fence_after_sync();
-      const uint32_t taddr = tmem_base + part * NT + (static_cast<uint32_t>(quarter * 32) << 16);
+      uint32_t v[T::kCols];
+      tmem_ld_columns(tmem_base + part * NT + col + (static_cast<uint32_t>(quarter * 32) << 16), v);
+      uint64_t s[T::kCols / 2];
 #pragma unroll
-      for (int c = 0; c < NT; c += T::kChunk) {
-        uint32_t v[T::kChunk];
-        tmem_ld_columns(taddr + c, v);
-        float s[T::kChunk];
-#pragma unroll
-        for (int j = 0; j < T::kChunk / 4; ++j) {
-          uint4 raw;
-          ptx::ld_shared_v4(scale_base + part * T::kScaleBytes + (c + 4 * j) * 4, raw);
-          s[4 * j] = __uint_as_float(raw.x); s[4 * j + 1] = __uint_as_float(raw.y);
-          s[4 * j + 2] = __uint_as_float(raw.z); s[4 * j + 3] = __uint_as_float(raw.w);
-        }
-        tmem_wait(v);
-#pragma unroll
-        for (int j = 0; j < T::kChunk; ++j) acc[c + j] = fmaf(__uint_as_float(v[j]), s[j], acc[c + j]);
+      for (int j = 0; j < T::kCols / 4; ++j) {
+        uint4 raw;
+        ptx::ld_shared_v4(scale_base + part * T::kScaleBytes + (col + 4 * j) * 4, raw);
+        s[2 * j] = pack_f32x2(raw.x, raw.y);
+        s[2 * j + 1] = pack_f32x2(raw.z, raw.w);
       }
+      tmem_wait(v);
+#pragma unroll
+      for (int j = 0; j < T::kCols / 2; ++j) fma_f32x2(acc[j], pack_f32x2(v[2 * j], v[2 * j + 1]), s[j]);
       ptx::tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(bar_part_empty + 8 * part);
@@ -735,55 +739,54 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
       }
     }
   }
-  // Every product of this CTA has been formed and read: the stages are free for the exchange.  [token][weight row].
-  if (warp >= 4) {
+  __syncwarp();
+  ptx::cluster_wait();
+  const int tokens_each = NT >> split_bits;  // room per CTA in every owner's memory
+  if (warp >= 4 && ok) {
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      asm volatile("st.shared.f32 [%0], %1;" ::"r"(smem_base + (j * kBM + row) * 4), "f"(acc[j]) : "memory");
+    for (int j = 0; j < T::kCols; ++j) {
+      const int token = col + j;
+      if (token < tokens) {
+        float lo, hi;
+        unpack_f32x2(acc[j / 2], lo, hi);
+        const uint32_t dst = ptx::map_to_cta(sums + ((rank * tokens_each + (token >> split_bits)) * kBM + row) * 4,
+                                             static_cast<uint32_t>(token & (splits - 1)));
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"((j & 1) ? hi : lo) : "memory");
+      }
     }
   }
   __syncwarp();
-  ptx::cluster_sync();
-  // This CTA's share of the tokens, summed over the CTAs in their order: a thread takes four neighbouring columns of
-  // a token, a warp a token at a time (every warp of the CTA), and asks for all CTAs' pieces before it adds them.
+  ptx::cluster_sync();  // all pieces are in place; nobody touches another CTA's memory after this
+  // A thread takes four neighbouring columns of a token, a warp a token at a time (every warp of the CTA).
   if (*abort_flag == 0) {
     const int col0 = n0 + 4 * lane;
     const bool four = col0 + 4 <= g.n && g.out_kind == LC0B200_OUT_BF16 && (g.ldc % 4) == 0 &&
                       (reinterpret_cast<uintptr_t>(g.out) % 8) == 0;
-    for (int j = tokens * rank / splits + warp; j < tokens * (rank + 1) / splits; j += T::kThreads / 32) {
-      float piece[kMaxSplits][4];
-#pragma unroll
-      for (int r = 0; r < kMaxSplits; ++r) {
-        if (r < splits) {
-          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                       : "=f"(piece[r][0]), "=f"(piece[r][1]), "=f"(piece[r][2]), "=f"(piece[r][3])
-                       : "r"(ptx::map_to_cta(smem_base + (j * kBM + 4 * lane) * 4, static_cast<uint32_t>(r)))
-                       : "memory");
-        }
+    for (int i = warp; rank + (i << split_bits) < tokens; i += T::kThreads / 32) {
+      float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int r = 0; r < splits; ++r) {
+        uint4 piece;
+        ptx::ld_shared_v4(sums + ((r * tokens_each + i) * kBM + 4 * lane) * 4, piece);
+        y[0] += __uint_as_float(piece.x);
+        y[1] += __uint_as_float(piece.y);
+        y[2] += __uint_as_float(piece.z);
+        y[3] += __uint_as_float(piece.w);
       }
-      float y[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float sum = piece[0][i];
-#pragma unroll
-        for (int r = 1; r < kMaxSplits; ++r) {
-          if (r < splits) sum += piece[r][i];
-        }
-        y[i] = col0 + i < g.n ? finish_one(sum, g, col0 + i) : 0.0f;
+      for (int c = 0; c < 4; ++c) {
+        if (col0 + c < g.n) y[c] = finish_one(y[c], g, col0 + c);
       }
-      const long long at = (m0 + j) * g.ldc + col0;
+      const long long at = (m0 + rank + (i << split_bits)) * g.ldc + col0;
       if (four) {
         *reinterpret_cast<uint2*>(reinterpret_cast<bf16*>(g.out) + at) = make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
       } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (col0 + i < g.n) store_one(y[i], g, at + i);
+        for (int c = 0; c < 4; ++c) {
+          if (col0 + c < g.n) store_one(y[c], g, at + c);
         }
       }
     }
   }
-  __syncwarp();
-  ptx::cluster_sync();  // nobody leaves while its sums may still be read
 
   ptx::tc_fence_before_sync();
   __syncthreads();
