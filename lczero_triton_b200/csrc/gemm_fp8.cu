@@ -525,8 +525,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
 // mostly padding.  So the roles are turned round: 128 weight rows are the M side of the MMA, NT = 16, 32 or 64 tokens its
 // N side, and out^T comes out: an epilogue thread owns one weight row, a block's scales are one product per token.  The k
 // blocks of a tile are split over the CTAs of a cluster, so that a layer of a few tiles still pulls on the memory of every
-// SM.  Token j is finished by CTA j mod S: each CTA writes its sums for it straight into that CTA's shared memory, one
-// cluster barrier later the owner adds the S pieces in the order of the CTAs (the same bits every time) and stores.
+// SM.  Tokens 4 i .. 4 i + 3 are finished by CTA i mod S: each CTA writes its sums for them straight into that CTA's
+// shared memory, one cluster barrier later the owner adds the S pieces in the order of the CTAs (the same bits every time).
 // (Fetching the pieces from the other CTAs instead took 2600 cycles a token and a second barrier of 2000.)  A CTA takes half
 // of an SM's shared memory and registers: two are resident, one loads while the other finishes.
 constexpr int kMaxSplits = 8;  // CTAs of a cluster (the portable limit)
@@ -543,7 +543,9 @@ struct Few {
   static constexpr int kThreads = 128 + 32 * kEpilogueWarps;  // in front: loads, MMAs, two for scales
   static constexpr int kBarrierBytes = 512;
   static constexpr int kScaleBytes = NT * 4;
-  static constexpr int kSumBytes = NT * kBM * 4;  // what the CTAs of a cluster write here: [CTA][token / S][weight row] f32
+  // What the CTAs of a cluster write here: [CTA][own groups of four tokens][weight row][4] f32.  A CTA owns one group at the
+  // least, also where there are more CTAs than groups.
+  static constexpr int kSumBytes = (NT / 4 > kMaxSplits ? NT / 4 : kMaxSplits) * kBM * 16;
   static constexpr int kFixedBytes = kSumBytes + kBarrierBytes + kPartials * kScaleBytes;
   static constexpr int kStages = (113 * 1024 - kFixedBytes) / kStageBytes;
   static_assert(kStages >= 3 && kStages <= 8, "pipeline depth");
@@ -741,48 +743,42 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
   }
   __syncwarp();
   ptx::cluster_wait();
-  const int tokens_each = NT >> split_bits;  // room per CTA in every owner's memory
+  // Groups of four tokens that a CTA may own; a piece of a group is one 16-byte word per weight row.
+  const int groups_each = max(1, (NT / 4) >> split_bits);
   if (warp >= 4 && ok) {
 #pragma unroll
-    for (int j = 0; j < T::kCols; ++j) {
-      const int token = col + j;
-      if (token < tokens) {
-        float lo, hi;
-        unpack_f32x2(acc[j / 2], lo, hi);
-        const uint32_t dst = ptx::map_to_cta(sums + ((rank * tokens_each + (token >> split_bits)) * kBM + row) * 4,
-                                             static_cast<uint32_t>(token & (splits - 1)));
-        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"((j & 1) ? hi : lo) : "memory");
+    for (int j = 0; j < T::kCols; j += 4) {
+      const int group = (col + j) / 4;
+      if (4 * group < tokens) {
+        const uint32_t dst = ptx::map_to_cta(sums + ((rank * groups_each + (group >> split_bits)) * kBM + row) * 16,
+                                             static_cast<uint32_t>(group & (splits - 1)));
+        asm volatile("st.shared::cluster.v2.b64 [%0], {%1, %2};" ::"r"(dst), "l"(acc[j / 2]), "l"(acc[j / 2 + 1]) : "memory");
       }
     }
   }
   __syncwarp();
   ptx::cluster_sync();  // all pieces are in place; nobody touches another CTA's memory after this
-  // A thread takes four neighbouring columns of a token, a warp a token at a time (every warp of the CTA).
+  // A warp takes 32 weight rows of a group at a time (every warp of the CTA), a lane one row: a column of the result.
   if (*abort_flag == 0) {
-    const int col0 = n0 + 4 * lane;
-    const bool four = col0 + 4 <= g.n && g.out_kind == LC0B200_OUT_BF16 && (g.ldc % 4) == 0 &&
-                      (reinterpret_cast<uintptr_t>(g.out) % 8) == 0;
-    for (int i = warp; rank + (i << split_bits) < tokens; i += T::kThreads / 32) {
+    for (int unit = warp;; unit += T::kThreads / 32) {
+      const int slot = unit >> 2;
+      const int token = 4 * ((slot << split_bits) + rank);
+      if (token >= tokens) break;
+      const int weight_row = (unit & 3) * 32 + lane;
+      const int column = n0 + weight_row;
       float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
       for (int r = 0; r < splits; ++r) {
         uint4 piece;
-        ptx::ld_shared_v4(sums + ((r * tokens_each + i) * kBM + 4 * lane) * 4, piece);
+        ptx::ld_shared_v4(sums + ((r * groups_each + slot) * kBM + weight_row) * 16, piece);
         y[0] += __uint_as_float(piece.x);
         y[1] += __uint_as_float(piece.y);
         y[2] += __uint_as_float(piece.z);
         y[3] += __uint_as_float(piece.w);
       }
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        if (col0 + c < g.n) y[c] = finish_one(y[c], g, col0 + c);
-      }
-      const long long at = (m0 + rank + (i << split_bits)) * g.ldc + col0;
-      if (four) {
-        *reinterpret_cast<uint2*>(reinterpret_cast<bf16*>(g.out) + at) = make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
-      } else {
+      if (column < g.n) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          if (col0 + c < g.n) store_one(y[c], g, at + c);
+          if (token + c < tokens) store_one(finish_one(y[c], g, column), g, (m0 + token + c) * g.ldc + column);
         }
       }
     }
@@ -896,14 +892,15 @@ int gemm_fp8(const GemmFp8& given, cudaStream_t stream) {
   if (g.m == 1) g.lda = ceil_div_ll(g.k, 16) * 16;
   if (g.n == 1) g.ldw = ceil_div_ll(g.k, 16) * 16;
   if (!aligned16(g.a) || !aligned16(g.w) || (g.lda % 16) != 0 || (g.ldw % 16) != 0) return gemm_fp8_simt(g, stream);
-  if (g.m <= 16) return launch_few<16>(g, stream);
-  if (g.m <= 32) return launch_few<32>(g, stream);
-  if (g.m <= 64) return launch_few<64>(g, stream);
-  // The widest tile that still gives most SMs one.
-  const long long enough = sm_count() * 3LL / 5;
-  if (2 * ceil_div_ll(g.m, 2 * kBM) * ceil_div_ll(g.n, 256) >= enough) return launch<256, 2>(g, stream);
-  if (ceil_div_ll(g.m, kBM) * ceil_div_ll(g.n, 128) >= enough) return launch<128, 1>(g, stream);
-  return launch_few<64>(g, stream);
+  // The widest tile that still gives most SMs one; then few-row tiles, the widest that make 60 of them (or the narrowest).
+  // (64 rows, 1536 x 1024: 4.2 us on 16-token tiles, 4.6 on 32, 6.3 on 64; 64 rows, 8192 x 8192: 25.6, 18.2, 17.3.)
+  const long long enough = sm_count() * 3LL / 5, some = sm_count() * 2LL / 5;
+  auto tiles = [&](int rows, int columns) { return ceil_div_ll(g.m, rows) * ceil_div_ll(g.n, columns); };
+  if (g.m > 64 && 2 * tiles(2 * kBM, 256) >= enough) return launch<256, 2>(g, stream);
+  if (g.m > 64 && tiles(kBM, 128) >= enough) return launch<128, 1>(g, stream);
+  if (g.m > 32 && tiles(64, kBM) >= some) return launch_few<64>(g, stream);
+  if (g.m > 16 && tiles(32, kBM) >= some) return launch_few<32>(g, stream);
+  return launch_few<16>(g, stream);
 }
 
 }  // namespace lc0b200
