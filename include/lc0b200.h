@@ -276,7 +276,8 @@ LC0B200_API int lc0b200_linear_int8_static(void* out_bf16, const void* a_bf16, c
  * The last block of a row (and the last rows of a matrix) may be short.  Scales of activations are block-major like the
  * row statistics of lc0b200_gemm: scale[block * ld_scale + row], ld_scale >= rows; scales of weights are
  * scale[(row / 128) * ld_scale + column / 128].  All ld* are row pitches in elements.  Outputs may not overlap inputs
- * except where said.  Bytes between a row's width and its pitch are neither read nor written. */
+ * except where said.  Bytes between a row's width and its pitch are never
+ * written; they may be read, and are ignored. */
 
 /* bf16 rows to codes; block_rows is 1 (activations) or 128 (weights, at load time).  Any alignment; 16-byte aligned
  * input rows and 8-byte aligned output rows are the fast form. */

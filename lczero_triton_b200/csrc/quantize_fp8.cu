@@ -6,6 +6,7 @@
 #include "common.cuh"
 #include "fp8.cuh"
 #include "kernels.h"
+#include "rows.cuh"
 
 namespace lc0b200 {
 
@@ -14,19 +15,6 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kRowsPerCta = kThreads / 16;  // a half-warp (16 lanes x 8 values) holds one 1 x 128 block
 
-// Eight bf16 values of a row from column `col`; what lies past the row's end reads as zero.
-template <bool VEC>
-__device__ __forceinline__ uint4 load8(const bf16* row, int col, int width) {
-  const int valid = width - col;
-  if (VEC && valid >= 8) return __ldg(reinterpret_cast<const uint4*>(row + col));
-  uint32_t w[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    if (j < valid) w[j >> 1] |= static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t*>(row) + col + j)) << (16 * (j & 1));
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
 // Magnitudes of bf16 values order as 16-bit unsigned integers (NaN above infinity): packed maximum of eight.
 __device__ __forceinline__ uint32_t packed_magnitude(const uint4& raw) {
   return __vmaxu2(__vmaxu2(raw.x & 0x7FFF7FFFu, raw.y & 0x7FFF7FFFu), __vmaxu2(raw.z & 0x7FFF7FFFu, raw.w & 0x7FFF7FFFu));
@@ -34,13 +22,13 @@ __device__ __forceinline__ uint32_t packed_magnitude(const uint4& raw) {
 // The larger half of a packed maximum as float bits.
 __device__ __forceinline__ uint32_t magnitude_of_packed(uint32_t m) { return max(m & 0xFFFFu, m >> 16) << 16; }
 
-template <bool VEC>
-__device__ __forceinline__ void store8(uint8_t* row, int col, int width, const uint4& raw, float inverse) {
+template <bool WORDS>
+__device__ __forceinline__ void store_codes(uint8_t* row, int col, int width, const uint4& raw, float inverse) {
   const float2 a = unpack_bf16x2(raw.x), b = unpack_bf16x2(raw.y), c = unpack_bf16x2(raw.z), d = unpack_bf16x2(raw.w);
   const uint32_t lo = fp8_pack4(a.x * inverse, a.y * inverse, b.x * inverse, b.y * inverse);
   const uint32_t hi = fp8_pack4(c.x * inverse, c.y * inverse, d.x * inverse, d.y * inverse);
   const int valid = width - col;
-  if (VEC && valid >= 8) {
+  if (WORDS && valid >= 8) {
     *reinterpret_cast<uint2*>(row + col) = make_uint2(lo, hi);
     return;
   }
@@ -51,7 +39,7 @@ __device__ __forceinline__ void store8(uint8_t* row, int col, int width, const u
 }
 
 // A half-warp takes UNROLL neighbouring blocks of one row; a CTA 16 rows.
-template <int UNROLL, bool VEC>
+template <int UNROLL, bool ALIGNED, bool WORDS>
 __global__ void __launch_bounds__(kThreads)
 quantize_fp8_rows_kernel(uint8_t* __restrict__ q_out, float* __restrict__ scale_out, const bf16* __restrict__ x, long long rows,
                          int width, long long ld_in, long long ld_out, long long ld_scale) {
@@ -64,15 +52,16 @@ quantize_fp8_rows_kernel(uint8_t* __restrict__ q_out, float* __restrict__ scale_
   uint8_t* dst = q_out + row * ld_out;
   const int blocks = static_cast<int>(ceil_div_ll(width, kFp8Block));
   for (int first = blockIdx.y * UNROLL; first < blocks; first += gridDim.y * UNROLL) {
-    uint4 raw[UNROLL];
+    RowWords words[UNROLL];
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
-      const int block = first + u;
-      raw[u] = (row_ok && block < blocks) ? load8<VEC>(src, block * kFp8Block + lane16 * 8, width) : make_uint4(0u, 0u, 0u, 0u);
+      words[u].a = words[u].b = make_uint4(0u, 0u, 0u, 0u);
+      if (row_ok && first + u < blocks) words[u] = load_words<ALIGNED>(src, (first + u) * kFp8Block + lane16 * 8, width, x, x + (rows - 1) * ld_in + width);
     }
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
-      uint32_t m = packed_magnitude(raw[u]);
+      const uint4 raw = channels_of<ALIGNED>(words[u], src, (first + u) * kFp8Block + lane16 * 8, width);
+      uint32_t m = packed_magnitude(raw);
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
       float scale, inverse;
@@ -80,14 +69,14 @@ quantize_fp8_rows_kernel(uint8_t* __restrict__ q_out, float* __restrict__ scale_
       const int block = first + u;
       if (row_ok && block < blocks) {
         if (lane16 == 0) scale_out[block * ld_scale + row] = scale;
-        store8<VEC>(dst, block * kFp8Block + lane16 * 8, width, raw[u], inverse);
+        store_codes<WORDS>(dst, block * kFp8Block + lane16 * 8, width, raw, inverse);
       }
     }
   }
 }
 
 // One CTA per 128 x 128 tile: each half-warp holds eight rows of the tile.
-template <bool VEC>
+template <bool ALIGNED, bool WORDS>
 __global__ void __launch_bounds__(kThreads)
 quantize_fp8_tiles_kernel(uint8_t* __restrict__ q_out, float* __restrict__ scale_out, const bf16* __restrict__ x, long long rows,
                           int width, long long ld_in, long long ld_out, long long ld_scale) {
@@ -101,12 +90,16 @@ quantize_fp8_tiles_kernel(uint8_t* __restrict__ q_out, float* __restrict__ scale
   int parity = 0;
   for (long long tile = blockIdx.y; tile < row_tiles; tile += gridDim.y, parity ^= 1) {
     const long long row0 = tile * kFp8Block + (threadIdx.x >> 4);
-    uint4 raw[kRowsPerThread];
+    RowWords words[kRowsPerThread];
 #pragma unroll
     for (int i = 0; i < kRowsPerThread; ++i) {
       const long long row = row0 + i * kRowsPerCta;
-      raw[i] = row < rows ? load8<VEC>(x + row * ld_in, col, width) : make_uint4(0u, 0u, 0u, 0u);
+      words[i].a = words[i].b = make_uint4(0u, 0u, 0u, 0u);
+      if (row < rows) words[i] = load_words<ALIGNED>(x + row * ld_in, col, width, x, x + (rows - 1) * ld_in + width);
     }
+    uint4 raw[kRowsPerThread];
+#pragma unroll
+    for (int i = 0; i < kRowsPerThread; ++i) raw[i] = channels_of<ALIGNED>(words[i], x + (row0 + i * kRowsPerCta) * ld_in, col, width);
     uint32_t m = 0u;
 #pragma unroll
     for (int i = 0; i < kRowsPerThread; ++i) m = __vmaxu2(m, packed_magnitude(raw[i]));
@@ -121,7 +114,7 @@ quantize_fp8_tiles_kernel(uint8_t* __restrict__ q_out, float* __restrict__ scale
 #pragma unroll
     for (int i = 0; i < kRowsPerThread; ++i) {
       const long long row = row0 + i * kRowsPerCta;
-      if (row < rows) store8<VEC>(q_out + row * ld_out, col, width, raw[i], inverse);
+      if (row < rows) store_codes<WORDS>(q_out + row * ld_out, col, width, raw[i], inverse);
     }
   }
 }
@@ -132,29 +125,24 @@ int quantize_fp8(void* out, float* scale, const void* in, long long rows, int wi
                  long long ld_out, long long ld_scale, cudaStream_t st) {
   auto* q = reinterpret_cast<uint8_t*>(out);
   const auto* x = reinterpret_cast<const bf16*>(in);
-  const bool vec = aligned16(in) && (ld_in % 8) == 0 && (reinterpret_cast<uintptr_t>(out) % 8) == 0 && (ld_out % 8) == 0;
+  const bool aligned = aligned16(in) && (ld_in % 8) == 0 && (width % 8) == 0;
+  const bool words = (reinterpret_cast<uintptr_t>(out) % 8) == 0 && (ld_out % 8) == 0;
   const long long blocks = ceil_div_ll(width, kFp8Block);
   const dim3 threads(kThreads);
   if (block_rows == 1) {
     constexpr int kUnroll = 4;
-    const unsigned row_ctas = static_cast<unsigned>(ceil_div_ll(rows, kRowsPerCta));
-    auto columns = [&](long long groups) { return static_cast<unsigned>(groups < 65535 ? groups : 65535); };
-    if (vec) {
-      launch_dependent(quantize_fp8_rows_kernel<kUnroll, true>, dim3(row_ctas, columns(ceil_div_ll(blocks, kUnroll))), threads, 0, st,
-                       q, scale, x, rows, width, ld_in, ld_out, ld_scale);
-    } else {
-      launch_dependent(quantize_fp8_rows_kernel<1, false>, dim3(row_ctas, columns(blocks)), threads, 0, st, q, scale, x, rows,
-                       width, ld_in, ld_out, ld_scale);
-    }
+    const long long groups = ceil_div_ll(blocks, kUnroll);
+    const dim3 grid(static_cast<unsigned>(ceil_div_ll(rows, kRowsPerCta)), static_cast<unsigned>(groups < 65535 ? groups : 65535));
+    if (aligned && words) launch_dependent(quantize_fp8_rows_kernel<kUnroll, true, true>, grid, threads, 0, st, q, scale, x, rows, width, ld_in, ld_out, ld_scale);
+    else if (words) launch_dependent(quantize_fp8_rows_kernel<kUnroll, false, true>, grid, threads, 0, st, q, scale, x, rows, width, ld_in, ld_out, ld_scale);
+    else launch_dependent(quantize_fp8_rows_kernel<kUnroll, false, false>, grid, threads, 0, st, q, scale, x, rows, width, ld_in, ld_out, ld_scale);
     return launch_status();
   }
   const long long row_tiles = ceil_div_ll(rows, kFp8Block);
   const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(row_tiles < 65535 ? row_tiles : 65535));
-  if (vec) {
-    launch_dependent(quantize_fp8_tiles_kernel<true>, grid, threads, 0, st, q, scale, x, rows, width, ld_in, ld_out, ld_scale);
-  } else {
-    launch_dependent(quantize_fp8_tiles_kernel<false>, grid, threads, 0, st, q, scale, x, rows, width, ld_in, ld_out, ld_scale);
-  }
+  if (aligned && words) launch_dependent(quantize_fp8_tiles_kernel<true, true>, grid, threads, 0, st, q, scale, x, rows, width, ld_in, ld_out, ld_scale);
+  else if (words) launch_dependent(quantize_fp8_tiles_kernel<false, true>, grid, threads, 0, st, q, scale, x, rows, width, ld_in, ld_out, ld_scale);
+  else launch_dependent(quantize_fp8_tiles_kernel<false, false>, grid, threads, 0, st, q, scale, x, rows, width, ld_in, ld_out, ld_scale);
   return launch_status();
 }
 
