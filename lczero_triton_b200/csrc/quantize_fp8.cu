@@ -56,7 +56,7 @@ quantize_fp8_rows_kernel(uint8_t* __restrict__ q_out, float* __restrict__ scale_
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
       words[u].a = words[u].b = make_uint4(0u, 0u, 0u, 0u);
-      if (row_ok && first + u < blocks) words[u] = load_words<ALIGNED>(src, (first + u) * kFp8Block + lane16 * 8, width, x, x + (rows - 1) * ld_in + width);
+      if (row_ok && first + u < blocks) words[u] = load_words<ALIGNED>(src, (first + u) * kFp8Block + lane16 * 8, width, inner_row(row, rows, ld_in));
     }
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
@@ -95,7 +95,7 @@ quantize_fp8_tiles_kernel(uint8_t* __restrict__ q_out, float* __restrict__ scale
     for (int i = 0; i < kRowsPerThread; ++i) {
       const long long row = row0 + i * kRowsPerCta;
       words[i].a = words[i].b = make_uint4(0u, 0u, 0u, 0u);
-      if (row < rows) words[i] = load_words<ALIGNED>(x + row * ld_in, col, width, x, x + (rows - 1) * ld_in + width);
+      if (row < rows) words[i] = load_words<ALIGNED>(x + row * ld_in, col, width, inner_row(row, rows, ld_in));
     }
     uint4 raw[kRowsPerThread];
 #pragma unroll

@@ -58,23 +58,28 @@ __global__ void __launch_bounds__(THREADS == 32 ? 32 * kWarpsPerBlock : THREADS)
   grid_dependency_release();
   grid_dependency_wait();
   const int lane = threadIdx.x & 31;
-  const int t = THREADS == 32 ? lane : threadIdx.x;
+  // Group g of this thread starts at channel first + kStep g: a step of all threads, or, for rows that need shifting, of a
+  // warp, which then walks a run of its own (store8_row).
+  constexpr int kStep = 8 * (ALIGNED ? THREADS : 32);
+  const int warp_in_row = THREADS == 32 ? 0 : threadIdx.x >> 5;
+  const int warp_first = 256 * warp_in_row * (ALIGNED ? 1 : GROUPS);
+  const int first = warp_first + 8 * lane;
   const long long row = THREADS == 32 ? blockIdx.x * static_cast<long long>(kWarpsPerBlock) + (threadIdx.x >> 5) : blockIdx.x;
   if (THREADS == 32 && row >= p.rows) return;
   const bf16* x = p.x + row * p.ld_x;
   const bf16* skip = p.skip + row * p.ld_skip;
+  const bool inner = inner_row(row, p.rows, p.ld_x), inner_skip = SKIP && inner_row(row, p.rows, p.ld_skip);
   RowWords raw[GROUPS], raw_skip[GROUPS];
 #pragma unroll
   for (int g = 0; g < GROUPS; ++g) {
-    const int col = 8 * (t + THREADS * g);
-    raw[g] = load_words<ALIGNED>(x, col, p.width, p.x, p.x + (p.rows - 1) * p.ld_x + p.width);
-    if (SKIP) raw_skip[g] = load_words<ALIGNED>(skip, col, p.width, p.skip, p.skip + (p.rows - 1) * p.ld_skip + p.width);
+    raw[g] = load_words<ALIGNED>(x, first + kStep * g, p.width, inner);
+    if (SKIP) raw_skip[g] = load_words<ALIGNED>(skip, first + kStep * g, p.width, inner_skip);
   }
   float v[GROUPS][8];  // zeros past the row's end
   float sum = 0.0f;
 #pragma unroll
   for (int g = 0; g < GROUPS; ++g) {
-    const int col = 8 * (t + THREADS * g);
+    const int col = first + kStep * g;
     unpack8(channels_of<ALIGNED>(raw[g], x, col, p.width), v[g]);
     if (SKIP) {
       float s[8];
@@ -98,20 +103,26 @@ __global__ void __launch_bounds__(THREADS == 32 ? 32 * kWarpsPerBlock : THREADS)
   // Every thread of the row has its operands from here on (a lane may have read a word that holds its neighbour's channels):
   // results may lie over them.
   const float rstd = 1.0f / sqrtf(sum / static_cast<float>(p.width) + p.epsilon);
+  const bool gamma_words = ALIGNED || aligned16_dev(p.gamma);
+  uint4 carry_residual = make_uint4(0u, 0u, 0u, 0u), carry_out = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
   for (int g = 0; g < GROUPS; ++g) {
-    if (8 * THREADS * g >= p.width) break;  // the same for the whole row: the shuffles below have every lane
-    const int col = 8 * (t + THREADS * g);
-    if (SKIP && p.residual != nullptr) store8_row<ALIGNED>(p.residual + row * p.ld_residual, col, p.width, pack8(v[g]));
+    if (warp_first + kStep * g >= p.width) break;  // the same for the warp: the shuffles below have every lane
+    const int col = first + kStep * g;
+    const bool begin = g == 0, end = g + 1 == GROUPS;
+    if (SKIP && p.residual != nullptr) store8_row<ALIGNED>(p.residual + row * p.ld_residual, col, p.width, pack8(v[g]), carry_residual, begin, end);
+    uint4 gamma_raw = make_uint4(0u, 0u, 0u, 0u);
+    if (gamma_words && col + 8 <= p.width) gamma_raw = __ldg(reinterpret_cast<const uint4*>(p.gamma + col));
+    else if (!ALIGNED && col < p.width) gamma_raw = edge_word(p.gamma, col, p.width);
     float gamma[8];
-    unpack8(channels_of<ALIGNED>(load_words<ALIGNED>(p.gamma, col, p.width, p.gamma, p.gamma + p.width), p.gamma, col, p.width), gamma);
+    unpack8(gamma_raw, gamma);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[g][j] = ALIGNED || col + j < p.width ? v[g][j] * rstd * gamma[j] : 0.0f;
-    if (ALIGNED && col >= p.width) {  // (0 * rstd may be NaN, and these lanes share a block's maximum)
+    for (int j = 0; j < 8; ++j) v[g][j] = v[g][j] * rstd * gamma[j];
+    if (col + 8 > p.width) {  // (0 * rstd may be NaN, and these channels share a block's maximum)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[g][j] = 0.0f;
+      for (int j = 0; j < 8; ++j) v[g][j] = col + j < p.width ? v[g][j] : 0.0f;
     }
-    if (p.out != nullptr) store8_row<ALIGNED>(p.out + row * p.ld_out, col, p.width, pack8(v[g]));
+    if (p.out != nullptr) store8_row<ALIGNED>(p.out + row * p.ld_out, col, p.width, pack8(v[g]), carry_out, begin, end);
     if (QUANT) {
       uint32_t amax = 0u;
 #pragma unroll
