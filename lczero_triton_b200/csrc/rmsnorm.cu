@@ -29,7 +29,7 @@ struct RmsParams {
   const bf16* gamma;
   long long rows, ld_x, ld_skip, ld_out, ld_residual, ld_q, ld_scale;
   int width;
-  int q_words;  // rows of codes start at multiples of 8 bytes
+  int q_even;  // rows of codes start at even addresses
   float epsilon;
 };
 
@@ -37,6 +37,20 @@ __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
   return v;
+}
+
+// Sum over the 32 or 256 threads of a row.
+template <int THREADS>
+__device__ __forceinline__ float row_sum(float sum) {
+  sum = warp_sum(sum);
+  if (THREADS == 32) return sum;
+  __shared__ float warp_part[THREADS / 32];
+  if ((threadIdx.x & 31) == 0) warp_part[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  sum = 0.0f;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) sum += warp_part[w];
+  return sum;
 }
 
 __device__ __forceinline__ void unpack8(const uint4& raw, float (&f)[8]) {
@@ -50,101 +64,146 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
   return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
 }
 
-// Rows in registers as groups of eight channels, THREADS (32 or 256) threads a row: thread t holds groups t,
-// t + THREADS, ...  Sixteen neighbouring lanes hold one 128-block of the e4m3 output.  SKIP, QUANT and the alignment of
-// the rows are fixed at compile time, every load of the row is issued before any arithmetic.
-template <int GROUPS, int THREADS, bool SKIP, bool QUANT, bool ALIGNED>
+// Rows in registers as 16-byte groups of eight channels, THREADS (32 or 256) threads a row: thread t holds groups t,
+// t + THREADS, ...  Sixteen neighbouring lanes hold one 128-block of the e4m3 output.  SKIP and QUANT are fixed at compile
+// time, every load of the row is issued before any arithmetic.
+template <int GROUPS, int THREADS, bool SKIP, bool QUANT>
 __global__ void __launch_bounds__(THREADS == 32 ? 32 * kWarpsPerBlock : THREADS) rms_norm_kernel(const RmsParams p) {
   grid_dependency_release();
   grid_dependency_wait();
   const int lane = threadIdx.x & 31;
-  // Group g of this thread starts at channel first + kStep g: a step of all threads, or, for rows that need shifting, of a
-  // warp, which then walks a run of its own (store8_row).
-  constexpr int kStep = 8 * (ALIGNED ? THREADS : 32);
-  const int warp_in_row = THREADS == 32 ? 0 : threadIdx.x >> 5;
-  const int warp_first = 256 * warp_in_row * (ALIGNED ? 1 : GROUPS);
-  const int first = warp_first + 8 * lane;
+  const int t = THREADS == 32 ? lane : threadIdx.x;
   const long long row = THREADS == 32 ? blockIdx.x * static_cast<long long>(kWarpsPerBlock) + (threadIdx.x >> 5) : blockIdx.x;
   if (THREADS == 32 && row >= p.rows) return;
-  const bf16* x = p.x + row * p.ld_x;
-  const bf16* skip = p.skip + row * p.ld_skip;
-  const bool inner = inner_row(row, p.rows, p.ld_x), inner_skip = SKIP && inner_row(row, p.rows, p.ld_skip);
-  RowWords raw[GROUPS], raw_skip[GROUPS];
+  const int groups = p.width >> 3;
+  const uint4* x = reinterpret_cast<const uint4*>(p.x + row * p.ld_x);
+  const uint4* skip = reinterpret_cast<const uint4*>(p.skip + row * p.ld_skip);
+  uint4 raw[GROUPS], raw_skip[GROUPS];
 #pragma unroll
   for (int g = 0; g < GROUPS; ++g) {
-    raw[g] = load_words<ALIGNED>(x, first + kStep * g, p.width, inner);
-    if (SKIP) raw_skip[g] = load_words<ALIGNED>(skip, first + kStep * g, p.width, inner_skip);
+    const int idx = t + THREADS * g;
+    raw[g] = raw_skip[g] = make_uint4(0u, 0u, 0u, 0u);
+    if (idx < groups) {
+      raw[g] = x[idx];
+      if (SKIP) raw_skip[g] = skip[idx];
+    }
   }
-  float v[GROUPS][8];  // zeros past the row's end
+  float v[GROUPS][8];
   float sum = 0.0f;
 #pragma unroll
   for (int g = 0; g < GROUPS; ++g) {
-    const int col = first + kStep * g;
-    unpack8(channels_of<ALIGNED>(raw[g], x, col, p.width), v[g]);
+    unpack8(raw[g], v[g]);
     if (SKIP) {
       float s[8];
-      unpack8(channels_of<ALIGNED>(raw_skip[g], skip, col, p.width), s);
+      unpack8(raw_skip[g], s);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[g][j] += s[j];
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) sum = fmaf(v[g][j], v[g][j], sum);
   }
-  sum = warp_sum(sum);
-  if (THREADS > 32) {
-    __shared__ float warp_part[THREADS / 32];
-    if (lane == 0) warp_part[threadIdx.x >> 5] = sum;
-    __syncthreads();
-    sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) sum += warp_part[w];
-  }
-  __syncwarp();
-  // Every thread of the row has its operands from here on (a lane may have read a word that holds its neighbour's channels):
-  // results may lie over them.
+  sum = row_sum<THREADS>(sum);
   const float rstd = 1.0f / sqrtf(sum / static_cast<float>(p.width) + p.epsilon);
-  const bool gamma_words = ALIGNED || aligned16_dev(p.gamma);
-  uint4 carry_residual = make_uint4(0u, 0u, 0u, 0u), carry_out = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
   for (int g = 0; g < GROUPS; ++g) {
-    if (warp_first + kStep * g >= p.width) break;  // the same for the warp: the shuffles below have every lane
-    const int col = first + kStep * g;
-    const bool begin = g == 0, end = g + 1 == GROUPS;
-    if (SKIP && p.residual != nullptr) store8_row<ALIGNED>(p.residual + row * p.ld_residual, col, p.width, pack8(v[g]), carry_residual, begin, end);
-    uint4 gamma_raw = make_uint4(0u, 0u, 0u, 0u);
-    if (gamma_words && col + 8 <= p.width) gamma_raw = __ldg(reinterpret_cast<const uint4*>(p.gamma + col));
-    else if (!ALIGNED && col < p.width) gamma_raw = edge_word(p.gamma, col, p.width);
+    if (THREADS * g >= groups) break;  // the same for the whole row: the shuffles below have every lane
+    const int idx = t + THREADS * g;
+    const bool here = idx < groups;
+    if (SKIP && p.residual != nullptr && here) reinterpret_cast<uint4*>(p.residual + row * p.ld_residual)[idx] = pack8(v[g]);
     float gamma[8];
-    unpack8(gamma_raw, gamma);
+    unpack8(here ? __ldg(reinterpret_cast<const uint4*>(p.gamma) + idx) : make_uint4(0u, 0u, 0u, 0u), gamma);
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[g][j] = v[g][j] * rstd * gamma[j];
-    if (col + 8 > p.width) {  // (0 * rstd may be NaN, and these channels share a block's maximum)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[g][j] = col + j < p.width ? v[g][j] : 0.0f;
-    }
-    if (p.out != nullptr) store8_row<ALIGNED>(p.out + row * p.ld_out, col, p.width, pack8(v[g]), carry_out, begin, end);
+    if (p.out != nullptr && here) reinterpret_cast<uint4*>(p.out + row * p.ld_out)[idx] = pack8(v[g]);
     if (QUANT) {
       uint32_t amax = 0u;
 #pragma unroll
       for (int j = 0; j < 8; ++j) amax = max(amax, magnitude_bits(v[g][j]));
+      amax = here ? amax : 0u;  // (0 * rstd may be NaN)
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
       float scale, inverse;
       fp8_block_scale(amax, scale, inverse);
-      if (col < p.width) {
-        if ((lane & 15) == 0) p.scale[(col / kFp8Block) * p.ld_scale + row] = scale;
-        const uint32_t lo = fp8_pack4(v[g][0] * inverse, v[g][1] * inverse, v[g][2] * inverse, v[g][3] * inverse);
-        const uint32_t hi = fp8_pack4(v[g][4] * inverse, v[g][5] * inverse, v[g][6] * inverse, v[g][7] * inverse);
-        uint8_t* q = p.q + row * p.ld_q + col;
-        if (ALIGNED || (p.q_words && col + 8 <= p.width)) {
-          *reinterpret_cast<uint2*>(q) = make_uint2(lo, hi);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            if (col + j < p.width) q[j] = static_cast<uint8_t>((j < 4 ? lo : hi) >> (8 * (j & 3)));
-          }
-        }
+      if (here) {
+        if ((lane & 15) == 0) p.scale[(idx >> 4) * p.ld_scale + row] = scale;
+        reinterpret_cast<uint2*>(p.q + row * p.ld_q)[idx] =
+            make_uint2(fp8_pack4(v[g][0] * inverse, v[g][1] * inverse, v[g][2] * inverse, v[g][3] * inverse),
+                       fp8_pack4(v[g][4] * inverse, v[g][5] * inverse, v[g][6] * inverse, v[g][7] * inverse));
       }
+    }
+  }
+}
+
+// The same for rows of any alignment and width, pairs of channels a lane (rows.cuh): a warp holds STEPS steps of 64 channels,
+// two steps are a 128-block.
+template <int STEPS, int THREADS, bool SKIP, bool QUANT>
+__global__ void __launch_bounds__(THREADS == 32 ? 32 * kWarpsPerBlock : THREADS) rms_norm_pairs_kernel(const RmsParams p) {
+  grid_dependency_release();
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31;
+  const int run = THREADS == 32 ? 0 : 64 * STEPS * (threadIdx.x >> 5);
+  const long long row = THREADS == 32 ? blockIdx.x * static_cast<long long>(kWarpsPerBlock) + (threadIdx.x >> 5) : blockIdx.x;
+  if (THREADS == 32 && row >= p.rows) return;
+  const bf16* x = p.x + row * p.ld_x;
+  const bf16* skip = p.skip + row * p.ld_skip;
+  uint32_t wx[STEPS + 1], ws[STEPS + 1];
+  load_row_words<STEPS>(wx, x, run, p.width, inner_row(row, p.rows, p.ld_x));
+  if (SKIP) load_row_words<STEPS>(ws, skip, run, p.width, inner_row(row, p.rows, p.ld_skip));
+  const int half_x = row_half(x), half_skip = row_half(skip);
+  float2 v[STEPS];
+  float sum = 0.0f;
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) {
+    v[s] = make_float2(0.0f, 0.0f);
+    if (run + 64 * s < p.width) {  // the same for the warp, here and below: the shuffles have every lane
+      v[s] = unpack_bf16x2(row_pair<STEPS>(wx, s, half_x));
+      if (SKIP) {
+        const float2 t = unpack_bf16x2(row_pair<STEPS>(ws, s, half_skip));
+        v[s].x += t.x;
+        v[s].y += t.y;
+      }
+      if (run + 64 * s + 64 > p.width) {
+        const int c = run + 64 * s + 2 * lane;
+        if (c >= p.width) v[s].x = 0.0f;
+        if (c + 1 >= p.width) v[s].y = 0.0f;
+      }
+      sum = fmaf(v[s].x, v[s].x, fmaf(v[s].y, v[s].y, sum));
+    }
+  }
+  sum = row_sum<THREADS>(sum);
+  // Every thread of the row has its operands from here on (a lane may have read a word that holds its neighbour's channel):
+  // results may lie over them.
+  __syncwarp();
+  const float rstd = 1.0f / sqrtf(sum / static_cast<float>(p.width) + p.epsilon);
+  bf16* residual = p.residual + row * p.ld_residual;
+  bf16* out = p.out + row * p.ld_out;
+  const int half_residual = row_half(residual), half_out = row_half(out);
+  uint32_t carry_residual = 0u, carry_out = 0u;
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) {
+    if (run + 64 * s < p.width) {
+      const int c = run + 64 * s + 2 * lane;
+      if (SKIP && p.residual != nullptr) {
+        store_row_pair(residual, c, half_residual, p.width, pack_bf16x2(v[s].x, v[s].y), carry_residual, s == 0, s + 1 == STEPS);
+      }
+      const float2 gamma = make_float2(c < p.width ? __bfloat162float(p.gamma[c]) : 0.0f, c + 1 < p.width ? __bfloat162float(p.gamma[c + 1]) : 0.0f);
+      v[s].x = v[s].x * rstd * gamma.x;
+      v[s].y = v[s].y * rstd * gamma.y;
+      if (p.out != nullptr) store_row_pair(out, c, half_out, p.width, pack_bf16x2(v[s].x, v[s].y), carry_out, s == 0, s + 1 == STEPS);
+    }
+    if (QUANT && (s & 1) != 0 && run + 64 * (s - 1) < p.width) {
+      const int c = run + 64 * (s - 1) + 2 * lane;
+      uint32_t amax = 0u;  // (0 * rstd may be NaN: channels past the row's end stay out of it)
+      if (c < p.width) amax = magnitude_bits(v[s - 1].x);
+      if (c + 1 < p.width) amax = max(amax, magnitude_bits(v[s - 1].y));
+      if (c + 64 < p.width) amax = max(amax, magnitude_bits(v[s].x));
+      if (c + 65 < p.width) amax = max(amax, magnitude_bits(v[s].y));
+      float scale, inverse;
+      fp8_block_scale(__reduce_max_sync(0xFFFFFFFFu, amax), scale, inverse);
+      if (lane == 0) p.scale[(c / kFp8Block) * p.ld_scale + row] = scale;
+      uint8_t* q = p.q + row * p.ld_q;
+      store_code_pair(q, c, p.width, p.q_even, v[s - 1].x * inverse, v[s - 1].y * inverse);
+      store_code_pair(q, c + 64, p.width, p.q_even, v[s].x * inverse, v[s].y * inverse);
     }
   }
 }
@@ -205,17 +264,25 @@ __global__ void __launch_bounds__(kThreads) rms_norm_any_kernel(const RmsParams 
   }
 }
 
-template <int GROUPS, int THREADS, bool ALIGNED>
+template <int SIZE, int THREADS, bool ALIGNED>
 void launch_rows(const RmsParams& p, cudaStream_t st) {
   const dim3 grid(static_cast<unsigned>(THREADS == 32 ? ceil_div_ll(p.rows, kWarpsPerBlock) : p.rows));
   const dim3 block(THREADS == 32 ? 32 * kWarpsPerBlock : THREADS);
   const bool skip = p.skip != nullptr, quant = p.q != nullptr;
-  if (skip && quant) launch_dependent(rms_norm_kernel<GROUPS, THREADS, true, true, ALIGNED>, grid, block, 0, st, p);
-  else if (skip) launch_dependent(rms_norm_kernel<GROUPS, THREADS, true, false, ALIGNED>, grid, block, 0, st, p);
-  else if (quant) launch_dependent(rms_norm_kernel<GROUPS, THREADS, false, true, ALIGNED>, grid, block, 0, st, p);
-  else launch_dependent(rms_norm_kernel<GROUPS, THREADS, false, false, ALIGNED>, grid, block, 0, st, p);
+  if constexpr (ALIGNED) {
+    if (skip && quant) launch_dependent(rms_norm_kernel<SIZE, THREADS, true, true>, grid, block, 0, st, p);
+    else if (skip) launch_dependent(rms_norm_kernel<SIZE, THREADS, true, false>, grid, block, 0, st, p);
+    else if (quant) launch_dependent(rms_norm_kernel<SIZE, THREADS, false, true>, grid, block, 0, st, p);
+    else launch_dependent(rms_norm_kernel<SIZE, THREADS, false, false>, grid, block, 0, st, p);
+  } else {
+    if (skip && quant) launch_dependent(rms_norm_pairs_kernel<4 * SIZE, THREADS, true, true>, grid, block, 0, st, p);
+    else if (skip) launch_dependent(rms_norm_pairs_kernel<4 * SIZE, THREADS, true, false>, grid, block, 0, st, p);
+    else if (quant) launch_dependent(rms_norm_pairs_kernel<4 * SIZE, THREADS, false, true>, grid, block, 0, st, p);
+    else launch_dependent(rms_norm_pairs_kernel<4 * SIZE, THREADS, false, false>, grid, block, 0, st, p);
+  }
 }
 
+// SIZE of a row of up to 256 SIZE channels a warp: 16-byte groups a lane, or four steps of pairs each.
 template <bool ALIGNED>
 bool launch_held(const RmsParams& p, cudaStream_t st) {
   // One warp per row up to 2048 channels, but not where there are fewer rows than SMs: a CTA then shares the row out.
@@ -261,9 +328,10 @@ int rms_norm(void* out, void* residual, void* q_out, float* q_scale, const void*
   p.ld_scale = ld_scale;
   p.width = width;
   p.epsilon = epsilon;
-  p.q_words = (reinterpret_cast<uintptr_t>(q_out) % 8) == 0 && (ld_q % 8) == 0;
-  const bool aligned = (width % 8) == 0 && rows_aligned16(in, ld_in) && rows_aligned16(skip, ld_skip) && rows_aligned16(out, ld_out) &&
-                       rows_aligned16(residual, ld_residual) && aligned16(gamma) && p.q_words;
+  p.q_even = ((reinterpret_cast<uintptr_t>(q_out) | static_cast<unsigned long long>(ld_q)) & 1u) == 0;
+  const bool aligned = (width % 8) == 0 && rows_aligned16(in, ld_in) && rows_aligned16(skip, ld_skip) &&
+                       rows_aligned16(out, ld_out) && rows_aligned16(residual, ld_residual) && aligned16(gamma) &&
+                       (q_out == nullptr || ((reinterpret_cast<uintptr_t>(q_out) % 8) == 0 && (ld_q % 8) == 0));
   if (aligned ? launch_held<true>(p, st) : launch_held<false>(p, st)) return launch_status();
   launch_dependent(rms_norm_any_kernel, dim3(static_cast<unsigned>(rows)), dim3(kThreads), 0, st, p);
   return launch_status();

@@ -1,12 +1,10 @@
-// Eight neighbouring bf16 channels of a row per lane, whatever the row's alignment and width.  A row of odd width starts
-// anywhere in a 16-byte word; reading it two bytes at a time ran at a quarter of the memory bandwidth.  A lane instead reads
-// the two aligned words that hold its eight channels (its neighbour reads the second one too: the L1 serves it) and
-// shifts.  Such a word may reach over the row's ends into the pitch or the next row, where it is read and ignored; in the
-// first and last rows it could reach over the ends of the operand, and they are read channel by channel.  The loads
-// depend on nothing but addresses, so that a kernel can issue all of a row's before the first shift waits for one.
-// Stores shift the other way, the missing channels coming from the lane before, and touch nothing outside the row.
-// ALIGNED: rows start at 16-byte words and hold whole words (width a multiple of 8); then all of this is one access.
-// (These rows are bound by instructions: what is done once a row has a branch of its own, what is done once a word has none.)
+// Rows of bf16 that start at any two-byte boundary and have any width.  A warp walks a run of the row 64 channels a step;
+// in step s lane l holds the pair of channels c = run + 64 s + 2 l and c + 1.  Memory is touched in aligned four-byte words:
+// where the row starts in the middle of one, a lane's pair is the upper half of its own word and the lower half of the
+// next lane's, one shuffle and one funnel shift.  (Single channels ran at a quarter of the memory bandwidth; shifting
+// eight channels between 16-byte words took three times as many instructions as this and was bound by them.)
+// A word may hold one channel's room before the row or behind it, which is read and ignored; the rows where that could lie
+// outside the operand are read channel by channel.  Nothing outside the row is written.
 #pragma once
 
 #include <stdint.h>
@@ -15,113 +13,58 @@
 
 namespace lc0b200 {
 
-// Channels `by` .. `by` + 7 (0 <= by < 8) of the sixteen in a | b.
-__device__ __forceinline__ uint4 shift_channels(const uint4& a, const uint4& b, int by) {
-  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-  uint32_t t[6], u[5];
+// 1 where the row starts in the upper half of a four-byte word.
+__device__ __forceinline__ int row_half(const bf16* row) { return static_cast<int>((reinterpret_cast<uintptr_t>(row) >> 1) & 1u); }
+
+// Whether one channel's room on either side of the row lies within the operand.
+__device__ __forceinline__ bool inner_row(long long row, long long rows, long long ld) { return row > 0 && row + 1 < rows && ld > 0; }
+
+// The word of channels c - half, c - half + 1, whose own room is 0 <= channel < width.
+__device__ __forceinline__ uint32_t load_row_word(const bf16* row, int c, int half, int width, bool inner) {
+  if (c - half >= width) return 0u;
+  if (inner) return *reinterpret_cast<const uint32_t*>(row + c - half);
+  const uint16_t* channels = reinterpret_cast<const uint16_t*>(row);
+  const uint32_t lo = c - half >= 0 ? channels[c - half] : 0u;
+  const uint32_t hi = c - half + 1 < width ? channels[c - half + 1] : 0u;
+  return lo | (hi << 16);
+}
+
+// STEPS steps of words from channel `run` on, and the word behind them (lane 0's); plain loads: a result may lie over its operand.
+template <int STEPS>
+__device__ __forceinline__ void load_row_words(uint32_t (&w)[STEPS + 1], const bf16* row, int run, int width, bool inner) {
+  const int lane = threadIdx.x & 31, half = row_half(row);
 #pragma unroll
-  for (int i = 0; i < 6; ++i) t[i] = (by & 4) ? w[i + 2] : w[i];
-#pragma unroll
-  for (int i = 0; i < 5; ++i) u[i] = (by & 2) ? t[i + 1] : t[i];
-  const int bits = (by & 1) * 16;
-  return make_uint4(__funnelshift_r(u[0], u[1], bits), __funnelshift_r(u[1], u[2], bits), __funnelshift_r(u[2], u[3], bits),
-                    __funnelshift_r(u[3], u[4], bits));
+  for (int s = 0; s < STEPS; ++s) w[s] = load_row_word(row, run + 64 * s + 2 * lane, half, width, inner);
+  w[STEPS] = lane == 0 && half != 0 ? load_row_word(row, run + 64 * STEPS, half, width, inner) : 0u;
 }
 
-// Channels between a 16-byte boundary and a row's start.
-__device__ __forceinline__ int row_offset(const bf16* row) { return static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15u) >> 1); }
-
-struct RowWords {
-  uint4 a, b;
-};
-
-// The word at row + at, put together from the row's own channels.
-static __device__ __noinline__ uint4 edge_word(const bf16* row, int at, int width) {
-  uint32_t w[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    if (at + j >= 0 && at + j < width) w[j >> 1] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(row)[at + j]) << (16 * (j & 1));
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
+// The pair of step s; channels past the row's end hold anything.  Every lane takes part.
+template <int STEPS>
+__device__ __forceinline__ uint32_t row_pair(const uint32_t (&w)[STEPS + 1], int s, int half) {
+  const int lane = threadIdx.x & 31;
+  // Lane 31's next word is lane 0's of the next step: the source lane sends the one that its reader needs.
+  const uint32_t next = __shfl_sync(0xFFFFFFFFu, lane == 0 ? w[s + 1] : w[s], (lane + 1) & 31);
+  return __funnelshift_r(w[s], next, 16 * half);
 }
 
-// Whether a word that holds a channel of this row lies within the operand, wherever it starts: seven channels may stick out.
-__device__ __forceinline__ bool inner_row(long long row, long long rows, long long ld) {
-  return row * ld >= 7 && (rows - 1 - row) * ld >= 7;
-}
-
-// The words of channels col .. col + 7 (col a multiple of 8); `inner` from inner_row.  Plain loads: a result may lie over its operand.
-template <bool ALIGNED>
-__device__ __forceinline__ RowWords load_words(const bf16* row, int col, int width, bool inner) {
-  RowWords r;
-  r.a = r.b = make_uint4(0u, 0u, 0u, 0u);
-  const int at = ALIGNED ? col : col - row_offset(row);
-  if (ALIGNED || inner) {
-    if (col < width) r.a = *reinterpret_cast<const uint4*>(row + at);
-    if (!ALIGNED && at + 8 < width) r.b = *reinterpret_cast<const uint4*>(row + at + 8);
-  } else {
-    if (col < width) r.a = edge_word(row, at, width);
-    if (at + 8 < width) r.b = edge_word(row, at + 8, width);
-  }
-  return r;
-}
-
-// ... and the channels themselves, zeros past the row's end.
-template <bool ALIGNED>
-__device__ __forceinline__ uint4 channels_of(const RowWords& r, const bf16* row, int col, int width) {
-  if (ALIGNED) return r.a;
-  uint4 v = shift_channels(r.a, r.b, row_offset(row));
-  const int valid = width - col;
-  if (valid < 8) {
-    v.x &= valid >= 2 ? 0xFFFFFFFFu : (valid == 1 ? 0xFFFFu : 0u);
-    v.y &= valid >= 4 ? 0xFFFFFFFFu : (valid == 3 ? 0xFFFFu : 0u);
-    v.z &= valid >= 6 ? 0xFFFFFFFFu : (valid == 5 ? 0xFFFFu : 0u);
-    v.w &= valid == 7 ? 0xFFFFu : 0u;
-  }
-  return v;
-}
-
-__device__ __forceinline__ void store_channels(bf16* row, int col, const uint4& v, int first, int end) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    if (j >= first && j < end) reinterpret_cast<uint16_t*>(row)[col + j] = static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1)));
-  }
-}
-
-// Stores this lane's channels col .. col + 7 (lane i's col is lane 0's plus 8 i) as far as they lie inside the row.  Every
-// lane of the warp takes part.  A warp walks a run of the row, 256 channels a step: `carry` takes the last lane's channels
-// from one step to the next, `begin` and `end` mark the run's first and last step.
-template <bool ALIGNED>
-__device__ __forceinline__ void store8_row(bf16* row, int col, int width, const uint4& v, uint4& carry, bool begin, bool end) {
-  const int valid = width - col;
-  if (ALIGNED) {
-    if (valid > 0) *reinterpret_cast<uint4*>(row + col) = v;
-    return;
-  }
-  const int off = row_offset(row);
-  if (off == 0) {  // the same for the warp
-    if (valid >= 8) *reinterpret_cast<uint4*>(row + col) = v;
-    else store_channels(row, col, v, 0, valid);
+// Stores the pair of channels c, c + 1 as far as they lie in the row.  `carry` takes lane 31's pair to the next step; `begin`,
+// `end`: the first and last step of this warp's run.  Every lane takes part.
+__device__ __forceinline__ void store_row_pair(bf16* row, int c, int half, int width, uint32_t pair, uint32_t& carry, bool begin, bool end) {
+  uint16_t* channels = reinterpret_cast<uint16_t*>(row);
+  if (half == 0) {  // the same for the warp
+    if (c + 1 < width) *reinterpret_cast<uint32_t*>(row + c) = pair;
+    else if (c < width) channels[c] = static_cast<uint16_t>(pair);
     return;
   }
   const int lane = threadIdx.x & 31;
-  uint4 before;
-  before.x = __shfl_sync(0xFFFFFFFFu, v.x, (lane + 31) & 31);
-  before.y = __shfl_sync(0xFFFFFFFFu, v.y, (lane + 31) & 31);
-  before.z = __shfl_sync(0xFFFFFFFFu, v.z, (lane + 31) & 31);
-  before.w = __shfl_sync(0xFFFFFFFFu, v.w, (lane + 31) & 31);
-  const uint4 last = before;
-  if (lane == 0) before = carry;
-  carry = last;
-  if (valid <= 0) return;
-  // The aligned word that ends inside this lane's channels: the last `off` of the lane before, then its own.
-  const uint4 word = shift_channels(before, v, 8 - off);
+  const uint32_t turned = __shfl_sync(0xFFFFFFFFu, pair, (lane + 31) & 31);
+  const uint32_t before = lane == 0 ? carry : turned;
+  carry = turned;  // lane 0 now holds this step's lane 31
   const bool first = begin && lane == 0;
-  if (!first && valid + off >= 8) *reinterpret_cast<uint4*>(row + col - off) = word;
-  else store_channels(row, col - off, word, first ? off : 0, valid + off);
-  // The last `off` channels are the next lane's to store, where there is one.
-  if (valid <= 8 || (end && lane == 31)) store_channels(row, col, v, 8 - off, valid);
+  if (c < width && !first) *reinterpret_cast<uint32_t*>(row + c - 1) = __funnelshift_r(before, pair, 16);
+  else if (first && c < width) channels[c] = static_cast<uint16_t>(pair);
+  // A channel c + 1 that no other lane's word holds: the row's last, or the run's.
+  if ((c + 2 == width || (end && lane == 31)) && c + 1 < width) channels[c + 1] = static_cast<uint16_t>(pair >> 16);
 }
 
 }  // namespace lc0b200
