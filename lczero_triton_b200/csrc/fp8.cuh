@@ -38,17 +38,6 @@ __device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d
 
 __device__ __forceinline__ uint8_t fp8_one(float a) { return __nv_cvt_float_to_fp8(a, __NV_SATFINITE, __NV_E4M3); }
 
-// Codes of the channels c, c + 1 of a row as far as they lie in it; `even`: rows start at even addresses (c is even).
-__device__ __forceinline__ void store_code_pair(uint8_t* row, int c, int width, bool even, float a, float b) {
-  const uint16_t codes = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-  if (even && c + 1 < width) {
-    *reinterpret_cast<uint16_t*>(row + c) = codes;
-  } else {
-    if (c < width) row[c] = static_cast<uint8_t>(codes);
-    if (c + 1 < width) row[c + 1] = static_cast<uint8_t>(codes >> 8);
-  }
-}
-
 __device__ __forceinline__ float fp8_value(uint8_t code) {
   const __half_raw h = __nv_cvt_fp8_to_halfraw(code, __NV_E4M3);
   return __half2float(__half(h));

@@ -6,7 +6,6 @@
 #include "common.cuh"
 #include "fp8.cuh"
 #include "kernels.h"
-#include "rows.cuh"
 
 namespace lc0b200 {
 
@@ -64,41 +63,49 @@ quantize_fp8_rows_kernel(uint8_t* __restrict__ q_out, float* __restrict__ scale_
   }
 }
 
-// Rows of any alignment and width, pairs of channels a lane (rows.cuh): a warp takes UNROLL neighbouring blocks of a row.
+// Rows of any alignment and width: a warp takes UNROLL neighbouring blocks of a row, channel lane + 32 i of a block to a lane.
+// FULL: all of them lie inside the row, nothing is checked per channel.
+template <int UNROLL, bool FULL>
+__device__ __forceinline__ void quantize_run(uint8_t* dst, float* scales, long long ld_scale, const bf16* src, int run, int width) {
+  const int lane = threadIdx.x & 31;
+  const uint16_t* x = reinterpret_cast<const uint16_t*>(src) + run + lane;
+  uint8_t* q = dst + run + lane;
+  uint32_t raw[UNROLL][4];  // bf16 bits
+#pragma unroll
+  for (int u = 0; u < UNROLL; ++u) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = kFp8Block * u + 32 * i;
+      raw[u][i] = FULL || run + at + lane < width ? __ldg(x + at) : 0u;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < UNROLL; ++u) {
+    if (!FULL && run + kFp8Block * u >= width) break;  // the same for the warp
+    const uint32_t m = max(max(raw[u][0] & 0x7FFFu, raw[u][1] & 0x7FFFu), max(raw[u][2] & 0x7FFFu, raw[u][3] & 0x7FFFu));
+    float scale, inverse;
+    fp8_block_scale(__reduce_max_sync(0xFFFFFFFFu, m) << 16, scale, inverse);
+    if (lane == 0) scales[(run / kFp8Block + u) * ld_scale] = scale;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = kFp8Block * u + 32 * i;
+      if (FULL || run + at + lane < width) q[at] = fp8_one(__uint_as_float(raw[u][i] << 16) * inverse);
+    }
+  }
+}
+
 template <int UNROLL>
 __global__ void __launch_bounds__(kThreads)
-quantize_fp8_row_pairs_kernel(uint8_t* __restrict__ q_out, float* __restrict__ scale_out, const bf16* __restrict__ x, long long rows,
-                              int width, long long ld_in, long long ld_out, long long ld_scale, bool even) {
+quantize_fp8_odd_rows_kernel(uint8_t* __restrict__ q_out, float* __restrict__ scale_out, const bf16* __restrict__ x, long long rows,
+                             int width, long long ld_in, long long ld_out, long long ld_scale) {
   grid_dependency_release();
   grid_dependency_wait();
-  const int lane = threadIdx.x & 31;
   const long long row = blockIdx.x * static_cast<long long>(kThreads / 32) + (threadIdx.x >> 5);
   if (row >= rows) return;
-  const bf16* src = x + row * ld_in;
-  const int half = row_half(src);
-  const bool inner = inner_row(row, rows, ld_in);
-  for (long long run = blockIdx.y * static_cast<long long>(UNROLL * kFp8Block); run < width; run += gridDim.y * static_cast<long long>(UNROLL * kFp8Block)) {
-    uint32_t w[2 * UNROLL + 1];
-    load_row_words<2 * UNROLL>(w, src, static_cast<int>(run), width, inner);
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const int c = static_cast<int>(run) + kFp8Block * u + 2 * lane;
-      if (c - 2 * lane >= width) break;  // the same for the warp
-      uint32_t pair[2] = {row_pair<2 * UNROLL>(w, 2 * u, half), row_pair<2 * UNROLL>(w, 2 * u + 1, half)};
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (c + 64 * i + 1 >= width) pair[i] = c + 64 * i < width ? pair[i] & 0xFFFFu : 0u;
-      }
-      const uint32_t m = __vmaxu2(pair[0] & 0x7FFF7FFFu, pair[1] & 0x7FFF7FFFu);
-      float scale, inverse;
-      fp8_block_scale(__reduce_max_sync(0xFFFFFFFFu, magnitude_of_packed(m)), scale, inverse);
-      if (lane == 0) scale_out[(c / kFp8Block) * ld_scale + row] = scale;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float2 v = unpack_bf16x2(pair[i]);
-        store_code_pair(q_out + row * ld_out, c + 64 * i, width, even, v.x * inverse, v.y * inverse);
-      }
-    }
+  constexpr int kRun = UNROLL * kFp8Block;
+  for (int run = blockIdx.y * kRun; run < width; run += gridDim.y * kRun) {
+    if (run + kRun <= width) quantize_run<UNROLL, true>(q_out + row * ld_out, scale_out + row, ld_scale, x + row * ld_in, run, width);
+    else quantize_run<UNROLL, false>(q_out + row * ld_out, scale_out + row, ld_scale, x + row * ld_in, run, width);
   }
 }
 
@@ -146,49 +153,46 @@ quantize_fp8_tiles_kernel(uint8_t* __restrict__ q_out, float* __restrict__ scale
   }
 }
 
-// ... and for rows of any alignment and width: a warp holds sixteen rows of the tile, two steps of pairs each.
+// ... and for rows of any alignment and width: a warp holds every eighth row of the tile, channel lane + 32 i to a lane.
 __global__ void __launch_bounds__(kThreads)
-quantize_fp8_tile_pairs_kernel(uint8_t* __restrict__ q_out, float* __restrict__ scale_out, const bf16* __restrict__ x, long long rows,
-                               int width, long long ld_in, long long ld_out, long long ld_scale, bool even) {
+quantize_fp8_odd_tiles_kernel(uint8_t* __restrict__ q_out, float* __restrict__ scale_out, const bf16* __restrict__ x, long long rows,
+                              int width, long long ld_in, long long ld_out, long long ld_scale) {
   grid_dependency_release();
   grid_dependency_wait();
   __shared__ uint32_t warp_max[2][kThreads / 32];
-  constexpr int kRowsPerWarp = kFp8Block / (kThreads / 32);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int run = blockIdx.x * kFp8Block;
+  constexpr int kWarps = kThreads / 32, kRowsPerWarp = kFp8Block / kWarps;
+  const int c0 = blockIdx.x * kFp8Block + (threadIdx.x & 31);
   const long long row_tiles = ceil_div_ll(rows, kFp8Block);
   int parity = 0;
   for (long long tile = blockIdx.y; tile < row_tiles; tile += gridDim.y, parity ^= 1) {
-    const long long row0 = tile * kFp8Block + warp;  // then every eighth
-    uint32_t w[kRowsPerWarp][3];
+    const long long row0 = tile * kFp8Block + (threadIdx.x >> 5);
+    uint32_t raw[kRowsPerWarp][2];  // bf16 bits, two channels to a word
+    uint32_t m = 0u;
 #pragma unroll
-    for (int i = 0; i < kRowsPerWarp; ++i) {
-      const long long row = row0 + 8 * i;
-      w[i][0] = w[i][1] = w[i][2] = 0u;
-      if (row < rows) load_row_words<2>(w[i], x + row * ld_in, run, width, inner_row(row, rows, ld_in));
+    for (int r = 0; r < kRowsPerWarp; ++r) {
+      const long long row = row0 + kWarps * r;
+      const uint16_t* src = reinterpret_cast<const uint16_t*>(x) + row * ld_in + c0;
+      uint32_t v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = row < rows && c0 + 32 * i < width ? __ldg(src + 32 * i) : 0u;
+      raw[r][0] = v[0] | (v[1] << 16);
+      raw[r][1] = v[2] | (v[3] << 16);
     }
-    uint32_t m = 0u, pair[kRowsPerWarp][2];
 #pragma unroll
-    for (int i = 0; i < kRowsPerWarp; ++i) {
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const int c = run + 64 * s + 2 * lane;
-        pair[i][s] = row_pair<2>(w[i], s, row_half(x + (row0 + 8 * i) * ld_in));
-        if (c + 1 >= width) pair[i][s] = c < width ? pair[i][s] & 0xFFFFu : 0u;
-        m = __vmaxu2(m, pair[i][s] & 0x7FFF7FFFu);
-      }
-    }
+    for (int r = 0; r < kRowsPerWarp; ++r) m = __vmaxu2(m, __vmaxu2(raw[r][0] & 0x7FFF7FFFu, raw[r][1] & 0x7FFF7FFFu));
     float scale, inverse;
     fp8_block_scale(cta_max(magnitude_of_packed(m), warp_max[parity]), scale, inverse);
     if (threadIdx.x == 0) scale_out[tile * ld_scale + blockIdx.x] = scale;
 #pragma unroll
-    for (int i = 0; i < kRowsPerWarp; ++i) {
-      const long long row = row0 + 8 * i;
+    for (int r = 0; r < kRowsPerWarp; ++r) {
+      const long long row = row0 + kWarps * r;
       if (row < rows) {
+        uint8_t* dst = q_out + row * ld_out + c0;
+        const float2 a = unpack_bf16x2(raw[r][0]), b = unpack_bf16x2(raw[r][1]);
+        const float v[4] = {a.x, a.y, b.x, b.y};
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const float2 v = unpack_bf16x2(pair[i][s]);
-          store_code_pair(q_out + row * ld_out, run + 64 * s + 2 * lane, width, even, v.x * inverse, v.y * inverse);
+        for (int i = 0; i < 4; ++i) {
+          if (c0 + 32 * i < width) dst[32 * i] = fp8_one(v[i] * inverse);
         }
       }
     }
@@ -202,7 +206,6 @@ int quantize_fp8(void* out, float* scale, const void* in, long long rows, int wi
   auto* q = reinterpret_cast<uint8_t*>(out);
   const auto* x = reinterpret_cast<const bf16*>(in);
   const bool aligned = (width % 8) == 0 && aligned16(in) && (ld_in % 8) == 0 && (reinterpret_cast<uintptr_t>(out) % 8) == 0 && (ld_out % 8) == 0;
-  const bool even = ((reinterpret_cast<uintptr_t>(out) | static_cast<unsigned long long>(ld_out)) & 1u) == 0;
   const long long blocks = ceil_div_ll(width, kFp8Block);
   const dim3 threads(kThreads);
   auto capped = [](long long count) { return static_cast<unsigned>(count < 65535 ? count : 65535); };
@@ -214,13 +217,13 @@ int quantize_fp8(void* out, float* scale, const void* in, long long rows, int wi
       launch_dependent(quantize_fp8_rows_kernel<kUnroll>, grid, threads, 0, st, q, scale, x, rows, width, ld_in, ld_out, ld_scale);
     } else {
       const dim3 grid(static_cast<unsigned>(ceil_div_ll(rows, kThreads / 32)), runs);
-      launch_dependent(quantize_fp8_row_pairs_kernel<kUnroll>, grid, threads, 0, st, q, scale, x, rows, width, ld_in, ld_out, ld_scale, even);
+      launch_dependent(quantize_fp8_odd_rows_kernel<kUnroll>, grid, threads, 0, st, q, scale, x, rows, width, ld_in, ld_out, ld_scale);
     }
     return launch_status();
   }
   const dim3 grid(static_cast<unsigned>(blocks), capped(ceil_div_ll(rows, kFp8Block)));
   if (aligned) launch_dependent(quantize_fp8_tiles_kernel, grid, threads, 0, st, q, scale, x, rows, width, ld_in, ld_out, ld_scale);
-  else launch_dependent(quantize_fp8_tile_pairs_kernel, grid, threads, 0, st, q, scale, x, rows, width, ld_in, ld_out, ld_scale, even);
+  else launch_dependent(quantize_fp8_odd_tiles_kernel, grid, threads, 0, st, q, scale, x, rows, width, ld_in, ld_out, ld_scale);
   return launch_status();
 }
 

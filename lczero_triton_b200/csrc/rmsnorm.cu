@@ -10,7 +10,6 @@
 #include "common.cuh"
 #include "fp8.cuh"
 #include "kernels.h"
-#include "rows.cuh"
 
 namespace lc0b200 {
 
@@ -29,7 +28,6 @@ struct RmsParams {
   const bf16* gamma;
   long long rows, ld_x, ld_skip, ld_out, ld_residual, ld_q, ld_scale;
   int width;
-  int q_even;  // rows of codes start at even addresses
   float epsilon;
 };
 
@@ -134,78 +132,89 @@ __global__ void __launch_bounds__(THREADS == 32 ? 32 * kWarpsPerBlock : THREADS)
   }
 }
 
-// The same for rows of any alignment and width, pairs of channels a lane (rows.cuh): a warp holds STEPS steps of 64 channels,
-// two steps are a 128-block.
-template <int STEPS, int THREADS, bool SKIP, bool QUANT>
-__global__ void __launch_bounds__(THREADS == 32 ? 32 * kWarpsPerBlock : THREADS) rms_norm_pairs_kernel(const RmsParams p) {
-  grid_dependency_release();
-  grid_dependency_wait();
-  const int lane = threadIdx.x & 31;
-  const int run = THREADS == 32 ? 0 : 64 * STEPS * (threadIdx.x >> 5);
-  const long long row = THREADS == 32 ? blockIdx.x * static_cast<long long>(kWarpsPerBlock) + (threadIdx.x >> 5) : blockIdx.x;
-  if (THREADS == 32 && row >= p.rows) return;
-  const bf16* x = p.x + row * p.ld_x;
-  const bf16* skip = p.skip + row * p.ld_skip;
-  uint32_t wx[STEPS + 1], ws[STEPS + 1];
-  load_row_words<STEPS>(wx, x, run, p.width, inner_row(row, p.rows, p.ld_x));
-  if (SKIP) load_row_words<STEPS>(ws, skip, run, p.width, inner_row(row, p.rows, p.ld_skip));
-  const int half_x = row_half(x), half_skip = row_half(skip);
-  float2 v[STEPS];
+// Rows of any alignment and width: a warp takes a run of 32 CHANNELS channels, channel run + lane + 32 i to a lane, so that
+// a warp's access is one run of memory and four channels of a lane make a 128-block; as many warps a row as it has runs.
+// Eight channels a lane keep many rows in flight: with a whole row of 1111 to a warp (48 channels a lane, 137 registers) 5003
+// rows took 27 us.  (16-byte or 4-byte words shifted into place move fewer requests and execute three times the instructions.)
+// FULL: the run lies inside the row, nothing is checked per channel.
+template <int CHANNELS, bool SKIP, bool FULL>
+__device__ __forceinline__ float load_run(const RmsParams& p, long long row, int c0, float (&v)[CHANNELS]) {
+  const bf16* x = p.x + row * p.ld_x + c0;
+  const bf16* skip = p.skip + row * p.ld_skip + c0;
+  bf16 raw[CHANNELS], raw_skip[CHANNELS];
+#pragma unroll
+  for (int i = 0; i < CHANNELS; ++i) {
+    raw[i] = raw_skip[i] = __ushort_as_bfloat16(0);
+    if (FULL || c0 + 32 * i < p.width) {
+      raw[i] = x[32 * i];
+      if (SKIP) raw_skip[i] = skip[32 * i];
+    }
+  }
   float sum = 0.0f;
 #pragma unroll
-  for (int s = 0; s < STEPS; ++s) {
-    v[s] = make_float2(0.0f, 0.0f);
-    if (run + 64 * s < p.width) {  // the same for the warp, here and below: the shuffles have every lane
-      v[s] = unpack_bf16x2(row_pair<STEPS>(wx, s, half_x));
-      if (SKIP) {
-        const float2 t = unpack_bf16x2(row_pair<STEPS>(ws, s, half_skip));
-        v[s].x += t.x;
-        v[s].y += t.y;
-      }
-      if (run + 64 * s + 64 > p.width) {
-        const int c = run + 64 * s + 2 * lane;
-        if (c >= p.width) v[s].x = 0.0f;
-        if (c + 1 >= p.width) v[s].y = 0.0f;
-      }
-      sum = fmaf(v[s].x, v[s].x, fmaf(v[s].y, v[s].y, sum));
+  for (int i = 0; i < CHANNELS; ++i) {
+    v[i] = __bfloat162float(raw[i]);
+    if (SKIP) v[i] += __bfloat162float(raw_skip[i]);
+    sum = fmaf(v[i], v[i], sum);
+  }
+  return sum;
+}
+
+template <int CHANNELS, bool SKIP, bool QUANT, bool FULL>
+__device__ __forceinline__ void store_run(const RmsParams& p, long long row, int c0, float (&v)[CHANNELS], float rstd) {
+  bf16* residual = p.residual + row * p.ld_residual + c0;
+  bf16* out = p.out + row * p.ld_out + c0;
+  if (SKIP && p.residual != nullptr) {
+#pragma unroll
+    for (int i = 0; i < CHANNELS; ++i) {
+      if (FULL || c0 + 32 * i < p.width) residual[32 * i] = __float2bfloat16_rn(v[i]);
     }
   }
-  sum = row_sum<THREADS>(sum);
-  // Every thread of the row has its operands from here on (a lane may have read a word that holds its neighbour's channel):
-  // results may lie over them.
-  __syncwarp();
-  const float rstd = 1.0f / sqrtf(sum / static_cast<float>(p.width) + p.epsilon);
-  bf16* residual = p.residual + row * p.ld_residual;
-  bf16* out = p.out + row * p.ld_out;
-  const int half_residual = row_half(residual), half_out = row_half(out);
-  uint32_t carry_residual = 0u, carry_out = 0u;
 #pragma unroll
-  for (int s = 0; s < STEPS; ++s) {
-    if (run + 64 * s < p.width) {
-      const int c = run + 64 * s + 2 * lane;
-      if (SKIP && p.residual != nullptr) {
-        store_row_pair(residual, c, half_residual, p.width, pack_bf16x2(v[s].x, v[s].y), carry_residual, s == 0, s + 1 == STEPS);
-      }
-      const float2 gamma = make_float2(c < p.width ? __bfloat162float(p.gamma[c]) : 0.0f, c + 1 < p.width ? __bfloat162float(p.gamma[c + 1]) : 0.0f);
-      v[s].x = v[s].x * rstd * gamma.x;
-      v[s].y = v[s].y * rstd * gamma.y;
-      if (p.out != nullptr) store_row_pair(out, c, half_out, p.width, pack_bf16x2(v[s].x, v[s].y), carry_out, s == 0, s + 1 == STEPS);
-    }
-    if (QUANT && (s & 1) != 0 && run + 64 * (s - 1) < p.width) {
-      const int c = run + 64 * (s - 1) + 2 * lane;
-      uint32_t amax = 0u;  // (0 * rstd may be NaN: channels past the row's end stay out of it)
-      if (c < p.width) amax = magnitude_bits(v[s - 1].x);
-      if (c + 1 < p.width) amax = max(amax, magnitude_bits(v[s - 1].y));
-      if (c + 64 < p.width) amax = max(amax, magnitude_bits(v[s].x));
-      if (c + 65 < p.width) amax = max(amax, magnitude_bits(v[s].y));
+  for (int i = 0; i < CHANNELS; ++i) {
+    const bool here = FULL || c0 + 32 * i < p.width;
+    v[i] = here ? v[i] * rstd * __bfloat162float(p.gamma[c0 + 32 * i]) : 0.0f;
+    if (p.out != nullptr && here) out[32 * i] = __float2bfloat16_rn(v[i]);
+  }
+  if (QUANT) {
+    uint8_t* q = p.q + row * p.ld_q + c0;
+#pragma unroll
+    for (int b = 0; b < CHANNELS; b += 4) {
+      const int block = c0 / kFp8Block + b / 4;  // (a lane's first channel is in the run's first block)
+      if (!FULL && block * kFp8Block >= p.width) break;
+      uint32_t amax = 0u;
+#pragma unroll
+      for (int i = b; i < b + 4; ++i) amax = max(amax, magnitude_bits(v[i]));
       float scale, inverse;
       fp8_block_scale(__reduce_max_sync(0xFFFFFFFFu, amax), scale, inverse);
-      if (lane == 0) p.scale[(c / kFp8Block) * p.ld_scale + row] = scale;
-      uint8_t* q = p.q + row * p.ld_q;
-      store_code_pair(q, c, p.width, p.q_even, v[s - 1].x * inverse, v[s - 1].y * inverse);
-      store_code_pair(q, c + 64, p.width, p.q_even, v[s].x * inverse, v[s].y * inverse);
+      if ((threadIdx.x & 31) == 0) p.scale[block * p.ld_scale + row] = scale;
+#pragma unroll
+      for (int i = b; i < b + 4; ++i) {
+        if (FULL || c0 + 32 * i < p.width) q[32 * i] = fp8_one(v[i] * inverse);
+      }
     }
   }
+}
+
+template <int CHANNELS, bool SKIP, bool QUANT>
+__global__ void __launch_bounds__(1024) rms_norm_odd_kernel(const RmsParams p) {
+  grid_dependency_release();
+  grid_dependency_wait();
+  __shared__ float warp_part[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long row = blockIdx.x;
+  const int c0 = 32 * CHANNELS * warp + lane;
+  const bool full = 32 * CHANNELS * (warp + 1) <= p.width;
+  float v[CHANNELS];
+  float sum = warp_sum(full ? load_run<CHANNELS, SKIP, true>(p, row, c0, v) : load_run<CHANNELS, SKIP, false>(p, row, c0, v));
+  if (blockDim.x > 32) {
+    if (lane == 0) warp_part[warp] = sum;
+    __syncthreads();
+    sum = warp_sum(lane < static_cast<int>(blockDim.x >> 5) ? warp_part[lane] : 0.0f);
+  }
+  const float rstd = 1.0f / sqrtf(sum / static_cast<float>(p.width) + p.epsilon);
+  if (full) store_run<CHANNELS, SKIP, QUANT, true>(p, row, c0, v, rstd);
+  else store_run<CHANNELS, SKIP, QUANT, false>(p, row, c0, v, rstd);
 }
 
 // Any width, pitch and alignment: one CTA per row, the row read twice (the second time from the caches).  Every value
@@ -264,43 +273,25 @@ __global__ void __launch_bounds__(kThreads) rms_norm_any_kernel(const RmsParams 
   }
 }
 
-template <int SIZE, int THREADS, bool ALIGNED>
-void launch_rows(const RmsParams& p, cudaStream_t st) {
+template <int GROUPS, int THREADS>
+void launch_words(const RmsParams& p, cudaStream_t st) {
   const dim3 grid(static_cast<unsigned>(THREADS == 32 ? ceil_div_ll(p.rows, kWarpsPerBlock) : p.rows));
   const dim3 block(THREADS == 32 ? 32 * kWarpsPerBlock : THREADS);
   const bool skip = p.skip != nullptr, quant = p.q != nullptr;
-  if constexpr (ALIGNED) {
-    if (skip && quant) launch_dependent(rms_norm_kernel<SIZE, THREADS, true, true>, grid, block, 0, st, p);
-    else if (skip) launch_dependent(rms_norm_kernel<SIZE, THREADS, true, false>, grid, block, 0, st, p);
-    else if (quant) launch_dependent(rms_norm_kernel<SIZE, THREADS, false, true>, grid, block, 0, st, p);
-    else launch_dependent(rms_norm_kernel<SIZE, THREADS, false, false>, grid, block, 0, st, p);
-  } else {
-    if (skip && quant) launch_dependent(rms_norm_pairs_kernel<4 * SIZE, THREADS, true, true>, grid, block, 0, st, p);
-    else if (skip) launch_dependent(rms_norm_pairs_kernel<4 * SIZE, THREADS, true, false>, grid, block, 0, st, p);
-    else if (quant) launch_dependent(rms_norm_pairs_kernel<4 * SIZE, THREADS, false, true>, grid, block, 0, st, p);
-    else launch_dependent(rms_norm_pairs_kernel<4 * SIZE, THREADS, false, false>, grid, block, 0, st, p);
-  }
+  if (skip && quant) launch_dependent(rms_norm_kernel<GROUPS, THREADS, true, true>, grid, block, 0, st, p);
+  else if (skip) launch_dependent(rms_norm_kernel<GROUPS, THREADS, true, false>, grid, block, 0, st, p);
+  else if (quant) launch_dependent(rms_norm_kernel<GROUPS, THREADS, false, true>, grid, block, 0, st, p);
+  else launch_dependent(rms_norm_kernel<GROUPS, THREADS, false, false>, grid, block, 0, st, p);
 }
 
-// SIZE of a row of up to 256 SIZE channels a warp: 16-byte groups a lane, or four steps of pairs each.
-template <bool ALIGNED>
-bool launch_held(const RmsParams& p, cudaStream_t st) {
-  // One warp per row up to 2048 channels, but not where there are fewer rows than SMs: a CTA then shares the row out.
-  const int width = p.width;
-  if (width <= 2048 && (p.rows > sm_count() || width <= 256)) {
-    if (width <= 256) launch_rows<1, 32, ALIGNED>(p, st);
-    else if (width <= 512) launch_rows<2, 32, ALIGNED>(p, st);
-    else if (width <= 1024) launch_rows<4, 32, ALIGNED>(p, st);
-    else if (width <= 1536) launch_rows<6, 32, ALIGNED>(p, st);
-    else launch_rows<8, 32, ALIGNED>(p, st);
-    return true;
-  }
-  if (width <= 2048) launch_rows<1, 256, ALIGNED>(p, st);
-  else if (width <= 4096) launch_rows<2, 256, ALIGNED>(p, st);
-  else if (width <= 8192) launch_rows<4, 256, ALIGNED>(p, st);
-  else if (width <= 16384) launch_rows<8, 256, ALIGNED>(p, st);
-  else return false;
-  return true;
+template <int CHANNELS>
+void launch_odd(const RmsParams& p, cudaStream_t st) {
+  const dim3 grid(static_cast<unsigned>(p.rows)), block(static_cast<unsigned>(32 * ceil_div_ll(p.width, 32 * CHANNELS)));
+  const bool skip = p.skip != nullptr, quant = p.q != nullptr;
+  if (skip && quant) launch_dependent(rms_norm_odd_kernel<CHANNELS, true, true>, grid, block, 0, st, p);
+  else if (skip) launch_dependent(rms_norm_odd_kernel<CHANNELS, true, false>, grid, block, 0, st, p);
+  else if (quant) launch_dependent(rms_norm_odd_kernel<CHANNELS, false, true>, grid, block, 0, st, p);
+  else launch_dependent(rms_norm_odd_kernel<CHANNELS, false, false>, grid, block, 0, st, p);
 }
 
 // 16-byte accesses to every row of a bf16 operand that is there.
@@ -328,11 +319,36 @@ int rms_norm(void* out, void* residual, void* q_out, float* q_scale, const void*
   p.ld_scale = ld_scale;
   p.width = width;
   p.epsilon = epsilon;
-  p.q_even = ((reinterpret_cast<uintptr_t>(q_out) | static_cast<unsigned long long>(ld_q)) & 1u) == 0;
-  const bool aligned = (width % 8) == 0 && rows_aligned16(in, ld_in) && rows_aligned16(skip, ld_skip) &&
-                       rows_aligned16(out, ld_out) && rows_aligned16(residual, ld_residual) && aligned16(gamma) &&
-                       (q_out == nullptr || ((reinterpret_cast<uintptr_t>(q_out) % 8) == 0 && (ld_q % 8) == 0));
-  if (aligned ? launch_held<true>(p, st) : launch_held<false>(p, st)) return launch_status();
+  const bool words = (width % 8) == 0 && rows_aligned16(in, ld_in) && rows_aligned16(skip, ld_skip) &&
+                     rows_aligned16(out, ld_out) && rows_aligned16(residual, ld_residual) && aligned16(gamma) &&
+                     (q_out == nullptr || ((reinterpret_cast<uintptr_t>(q_out) % 8) == 0 && (ld_q % 8) == 0));
+  if (words && width <= 16384) {
+    // One warp per row up to 2048 channels, but not where there are fewer rows than SMs: a CTA then shares the row out.
+    if (width <= 2048 && (rows > sm_count() || width <= 256)) {
+      if (width <= 256) launch_words<1, 32>(p, st);
+      else if (width <= 512) launch_words<2, 32>(p, st);
+      else if (width <= 1024) launch_words<4, 32>(p, st);
+      else if (width <= 1536) launch_words<6, 32>(p, st);
+      else launch_words<8, 32>(p, st);
+    } else if (width <= 2048) {
+      launch_words<1, 256>(p, st);
+    } else if (width <= 4096) {
+      launch_words<2, 256>(p, st);
+    } else if (width <= 8192) {
+      launch_words<4, 256>(p, st);
+    } else {
+      launch_words<8, 256>(p, st);
+    }
+    return launch_status();
+  }
+  if (width <= 8192) {
+    launch_odd<8>(p, st);
+    return launch_status();
+  }
+  if (width <= 16384) {
+    launch_odd<16>(p, st);
+    return launch_status();
+  }
   launch_dependent(rms_norm_any_kernel, dim3(static_cast<unsigned>(rows)), dim3(kThreads), 0, st, p);
   return launch_status();
 }
