@@ -37,12 +37,13 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// Sum over the 32 or 256 threads of a row.
+// Sum over the 16, 32 or 256 threads of a row.
 template <int THREADS>
 __device__ __forceinline__ float row_sum(float sum) {
-  sum = warp_sum(sum);
-  if (THREADS == 32) return sum;
-  __shared__ float warp_part[THREADS / 32];
+#pragma unroll
+  for (int o = THREADS < 32 ? THREADS / 2 : 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+  if (THREADS <= 32) return sum;
+  __shared__ float warp_part[THREADS < 32 ? 1 : THREADS / 32];
   if ((threadIdx.x & 31) == 0) warp_part[threadIdx.x >> 5] = sum;
   __syncthreads();
   sum = 0.0f;
@@ -62,18 +63,18 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
   return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
 }
 
-// Rows in registers as 16-byte groups of eight channels, THREADS (32 or 256) threads a row: thread t holds groups t,
+// Rows in registers as 16-byte groups of eight channels, THREADS (16, 32 or 256) threads a row: thread t holds groups t,
 // t + THREADS, ...  Sixteen neighbouring lanes hold one 128-block of the e4m3 output.  SKIP and QUANT are fixed at compile
 // time, every load of the row is issued before any arithmetic.
 template <int GROUPS, int THREADS, bool SKIP, bool QUANT>
-__global__ void __launch_bounds__(THREADS == 32 ? 32 * kWarpsPerBlock : THREADS) rms_norm_kernel(const RmsParams p) {
+__global__ void __launch_bounds__(THREADS == 32 ? 32 * kWarpsPerBlock : 256) rms_norm_kernel(const RmsParams p) {
   grid_dependency_release();
   grid_dependency_wait();
   const int lane = threadIdx.x & 31;
-  const int t = THREADS == 32 ? lane : threadIdx.x;
-  const long long row = THREADS == 32 ? blockIdx.x * static_cast<long long>(kWarpsPerBlock) + (threadIdx.x >> 5) : blockIdx.x;
+  const int t = threadIdx.x % THREADS;
+  const long long row = blockIdx.x * static_cast<long long>(blockDim.x / THREADS) + threadIdx.x / THREADS;
   if (THREADS == 32 && row >= p.rows) return;
-  const int groups = p.width >> 3;
+  const int groups = row < p.rows ? p.width >> 3 : 0;  // a half-warp without a row stays for the other half's shuffles
   const uint4* x = reinterpret_cast<const uint4*>(p.x + row * p.ld_x);
   const uint4* skip = reinterpret_cast<const uint4*>(p.skip + row * p.ld_skip);
   uint4 raw[GROUPS], raw_skip[GROUPS];
@@ -104,7 +105,7 @@ __global__ void __launch_bounds__(THREADS == 32 ? 32 * kWarpsPerBlock : THREADS)
   const float rstd = 1.0f / sqrtf(sum / static_cast<float>(p.width) + p.epsilon);
 #pragma unroll
   for (int g = 0; g < GROUPS; ++g) {
-    if (THREADS * g >= groups) break;  // the same for the whole row: the shuffles below have every lane
+    if (THREADS * g >= (p.width >> 3)) break;  // the same for every row: the shuffles below have every lane
     const int idx = t + THREADS * g;
     const bool here = idx < groups;
     if (SKIP && p.residual != nullptr && here) reinterpret_cast<uint4*>(p.residual + row * p.ld_residual)[idx] = pack8(v[g]);
@@ -275,8 +276,8 @@ __global__ void __launch_bounds__(kThreads) rms_norm_any_kernel(const RmsParams 
 
 template <int GROUPS, int THREADS>
 void launch_words(const RmsParams& p, cudaStream_t st) {
-  const dim3 grid(static_cast<unsigned>(THREADS == 32 ? ceil_div_ll(p.rows, kWarpsPerBlock) : p.rows));
-  const dim3 block(THREADS == 32 ? 32 * kWarpsPerBlock : THREADS);
+  const dim3 block(THREADS == 32 ? 32 * kWarpsPerBlock : 256);
+  const dim3 grid(static_cast<unsigned>(ceil_div_ll(p.rows, block.x / THREADS)));
   const bool skip = p.skip != nullptr, quant = p.q != nullptr;
   if (skip && quant) launch_dependent(rms_norm_kernel<GROUPS, THREADS, true, true>, grid, block, 0, st, p);
   else if (skip) launch_dependent(rms_norm_kernel<GROUPS, THREADS, true, false>, grid, block, 0, st, p);
@@ -325,7 +326,8 @@ int rms_norm(void* out, void* residual, void* q_out, float* q_scale, const void*
   if (words && width <= 16384) {
     // One warp per row up to 2048 channels, but not where there are fewer rows than SMs: a CTA then shares the row out.
     if (width <= 2048 && (rows > sm_count() || width <= 256)) {
-      if (width <= 256) launch_words<1, 32>(p, st);
+      if (width <= 128) launch_words<1, 16>(p, st);
+      else if (width <= 256) launch_words<1, 32>(p, st);
       else if (width <= 512) launch_words<2, 32>(p, st);
       else if (width <= 1024) launch_words<4, 32>(p, st);
       else if (width <= 1536) launch_words<6, 32>(p, st);

@@ -168,7 +168,7 @@ def _check_norm(x, skip, gamma, epsilon, out, residual, q, scale) -> None:
         assert bool((error <= allowed).all()), float((error / allowed).max())
 
 
-NORM_SHAPES = [(1, 1), (3, 8), (33, 31), (7, 128), (5, 130), (3, 1000), (64, 1024), (9, 1111), (5, 1536), (3, 2048), (4, 2056),
+NORM_SHAPES = [(1, 64), (15, 128), (16, 96), (17, 120), (1000, 32), (200, 136), (1, 1), (3, 8), (33, 31), (7, 128), (5, 130), (3, 1000), (64, 1024), (9, 1111), (5, 1536), (3, 2048), (4, 2056),
                (1, 4096), (3, 4100), (2, 8192), (2, 16384), (2, 16392), (1, 40000)]
 
 
