@@ -65,29 +65,6 @@ __device__ __forceinline__ float activate_rt(float x, int act) {
   }
 }
 
-// mish(x) = x * n / (n + 2) with n = e^x (e^x + 2) (reference formula: bt4/kernels/layer_norm.py:61-69,
-// which switches between n*q and x - 2q by range; with x clamped to <= 20 in the exponential the single
-// form is accurate everywhere: n / (n + 2) rounds to 1 from x = 9 on and tends to n / 2 for x -> -inf).
-// 32 values at a time; one reciprocal serves two elements (1/da = db / (da db)).  (Moving exponentials
-// to a polynomial on the FMA pipe was measured slower: every extra instruction issued by the epilogue
-// warps costs more than the transcendental unit saves.)
-__device__ __forceinline__ void mish32(float (&y)[32]) {
-  constexpr float kLog2e = 1.4426950408889634f;
-#pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    const float a = y[2 * j], b = y[2 * j + 1];
-    float ea, eb;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(ea) : "f"(fminf(a, 20.0f) * kLog2e));
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(eb) : "f"(fminf(b, 20.0f) * kLog2e));
-    const float na = ea * (ea + 2.0f), nb = eb * (eb + 2.0f);
-    const float da = na + 2.0f, db = nb + 2.0f;  // in [2, 2.4e17]: the product stays finite
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(da * db));
-    y[2 * j] = a * (na * (db * r));
-    y[2 * j + 1] = b * (nb * (da * r));
-  }
-}
-
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);

@@ -80,21 +80,6 @@ __device__ __forceinline__ void tmem_ld_columns(uint32_t taddr, uint32_t (&v)[16
 }
 __device__ __forceinline__ void tmem_ld_columns(uint32_t taddr, uint32_t (&v)[32]) { ptx::tmem_ld_32x32(taddr, v); }
 
-// A look at a barrier that never suspends.
-__device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n\t"
-      ".reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t"
-      "}\n"
-      : "=r"(done)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return done != 0;
-}
-
 __device__ __forceinline__ uint64_t pack_f32x2(uint32_t lo, uint32_t hi) {
   uint64_t r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
@@ -102,6 +87,17 @@ __device__ __forceinline__ uint64_t pack_f32x2(uint32_t lo, uint32_t hi) {
 }
 __device__ __forceinline__ void unpack_f32x2(uint64_t v, float& lo, float& hi) {
   asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t both_f32x2(float x) { return pack_f32x2(__float_as_uint(x), __float_as_uint(x)); }
+__device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 // acc += a * b, both halves.
 __device__ __forceinline__ void fma_f32x2(uint64_t& acc, uint64_t a, uint64_t b) {
@@ -161,8 +157,35 @@ __device__ __forceinline__ int mma_width(int n, int tile_n0) {
   return left >= BN ? BN : ((left + 31) & ~31);
 }
 
-// Bias and activation of 32 columns from col0 on; columns past the matrix edge get no bias (they are not stored).
-__device__ __forceinline__ void finish32(float (&y)[32], const GemmFp8& g, int col0) {
+// mish(x) = x n / (n + 2), n = e^x (e^x + 2) (formula: bt4/kernels/layer_norm.py:61-69), of two pairs at a time: packed
+// arithmetic, and one reciprocal for all four (1 / a = b c d / (a b c d)).  The exponential is taken of min(x, 11): there
+// n / (n + 2) rounds to 1, and the product of four denominators stays below 2e38.  What the transcendental unit does is
+// what this costs: five quarter-rate operations for four values instead of eight.
+__device__ __forceinline__ void mish4(uint64_t& xa, uint64_t& xb) {
+  const uint64_t two = both_f32x2(2.0f), log2e = both_f32x2(1.4426950408889634f);
+  auto power = [&](uint64_t x) {
+    float lo, hi, elo, ehi;
+    unpack_f32x2(mul_f32x2(x, log2e), lo, hi);
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(elo) : "f"(fminf(lo, 15.8696f)));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(ehi) : "f"(fminf(hi, 15.8696f)));
+    return pack_f32x2(__float_as_uint(elo), __float_as_uint(ehi));
+  };
+  const uint64_t ea = power(xa), eb = power(xb);
+  const uint64_t na = mul_f32x2(ea, add_f32x2(ea, two)), nb = mul_f32x2(eb, add_f32x2(eb, two));
+  const uint64_t da = add_f32x2(na, two), db = add_f32x2(nb, two);
+  float plo, phi, r;
+  unpack_f32x2(mul_f32x2(da, db), plo, phi);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(plo * phi));
+  const uint64_t rp = pack_f32x2(__float_as_uint(r * phi), __float_as_uint(r * plo));
+  xa = mul_f32x2(mul_f32x2(xa, na), mul_f32x2(rp, db));
+  xb = mul_f32x2(mul_f32x2(xb, nb), mul_f32x2(rp, da));
+}
+
+// Bias and activation of 32 columns from col0 on, as packed pairs; columns past the matrix edge get no bias (they are not
+// stored).  ACT is fixed at compile time: what a tile executes once has to be fetched once, and jumping over the other
+// activations cost 300 cycles for 32 columns that had nothing to do.
+template <int ACT>
+__device__ __forceinline__ void finish32(uint64_t (&y)[16], const GemmFp8& g, int col0) {
   if (g.bias != nullptr) {
     if (col0 + 32 <= g.n && aligned16_dev(g.bias)) {
 #pragma unroll
@@ -170,30 +193,44 @@ __device__ __forceinline__ void finish32(float (&y)[32], const GemmFp8& g, int c
         const uint4 raw = __ldg(reinterpret_cast<const uint4*>(g.bias + col0) + i);
         const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 b = unpack_bf16x2(words[j]);
-          y[8 * i + 2 * j] += b.x;
-          y[8 * i + 2 * j + 1] += b.y;
-        }
+        for (int j = 0; j < 4; ++j) y[4 * i + j] = add_f32x2(y[4 * i + j], pack_f32x2(words[j] << 16, words[j] & 0xFFFF0000u));
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < 32; ++j) y[j] += col0 + j < g.n ? __bfloat162float(g.bias[col0 + j]) : 0.0f;
+      for (int j = 0; j < 16; ++j) {
+        const int c = col0 + 2 * j;
+        y[j] = add_f32x2(y[j], pack_f32x2(__float_as_uint(c < g.n ? __bfloat162float(g.bias[c]) : 0.0f),
+                                          __float_as_uint(c + 1 < g.n ? __bfloat162float(g.bias[c + 1]) : 0.0f)));
+      }
     }
   }
-  // The activation is uniform for the launch: one branch per chunk, not per element.
-  if (g.activation == LC0B200_ACT_MISH) {
-    mish32(y);
-  } else if (g.activation == LC0B200_ACT_RELU) {
+  if (ACT == LC0B200_ACT_MISH) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) y[j] = y[j] < 0.0f ? 0.0f : y[j];  // NaN stays
-  } else if (g.activation == LC0B200_ACT_SWISH) {
+    for (int j = 0; j < 16; j += 2) mish4(y[j], y[j + 1]);
+  } else if (ACT != LC0B200_ACT_NONE) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) y[j] = act_swish(y[j]);
+    for (int j = 0; j < 16; ++j) {
+      float lo, hi;
+      unpack_f32x2(y[j], lo, hi);
+      if (ACT == LC0B200_ACT_RELU) {  // NaN stays
+        lo = lo < 0.0f ? 0.0f : lo;
+        hi = hi < 0.0f ? 0.0f : hi;
+      } else {
+        lo = act_swish(lo);
+        hi = act_swish(hi);
+      }
+      y[j] = pack_f32x2(__float_as_uint(lo), __float_as_uint(hi));
+    }
   }
 }
 
-template <int BN, int CTAS>
+__device__ __forceinline__ uint32_t pack_bf16x2(uint64_t pair) {
+  float lo, hi;
+  unpack_f32x2(pair, lo, hi);
+  return lc0b200::pack_bf16x2(lo, hi);
+}
+
+template <int BN, int CTAS, int ACT>
 __global__ void __launch_bounds__(Tile<BN, CTAS>::kThreads, 1)
 gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
                 const __grid_constant__ CUtensorMap map_out, const FpParams p) {
@@ -306,8 +343,9 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         const uint32_t idesc = ptx::instr_desc(1u, 0u, 0u, static_cast<uint32_t>(kTileM),
                                                static_cast<uint32_t>(mma_width<BN>(g.n, tile_n0)));
         for (int kb = 0; kb < k_blocks; ++kb) {
-          ok = ptx::mbar_wait(bar_part_empty + 8 * part, part_phase ^ 1u, abort_flag, p.status, 0x1200u + part);
-          ok = ok && ptx::mbar_wait(bar_full + 8 * stage, phase, abort_flag, p.status, 0x1300u + stage);
+          // The operands first: they are there early, and the look at their barrier is off the path from a freed partial.
+          ok = ptx::mbar_wait(bar_full + 8 * stage, phase, abort_flag, p.status, 0x1300u + stage);
+          ok = ok && ptx::mbar_wait(bar_part_empty + 8 * part, part_phase ^ 1u, abort_flag, p.status, 0x1200u + part);
           ok = __all_sync(0xFFFFFFFFu, ok);
           if (!ok) break;
           ptx::tc_fence_after_sync();
@@ -409,9 +447,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       // edge hold anything and are not stored.
       float scale = 0.0f, next_scale = 0.0f;
       uint32_t v[2][32];
-      bool ready = false;
       auto begin_block = [&](float& block_scale) {
-        if (!ready) ok = ptx::mbar_wait(bar_part_full + 8 * part, part_phase, abort_flag, p.status, 0x1400u + part);
+        ok = ptx::mbar_wait(bar_part_full + 8 * part, part_phase, abort_flag, p.status, 0x1400u + part);
         if (!ok) return;
         ptx::tc_fence_after_sync();
         ptx::tmem_ld_32x32(tmem_row + part * BN, v[0]);
@@ -425,14 +462,11 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
           part = 0;
           part_phase ^= 1u;
         }
-        ready = false;
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
           tmem_wait(v[c & 1]);
           if (c + 1 < kChunks) {
             ptx::tmem_ld_32x32(tmem_row + this_part * BN + 32 * (c + 1), v[(c + 1) & 1]);
-            // Look at the next partial's barrier while there is work to hide the look behind.
-            if (c + 2 == kChunks && kb + 1 < k_blocks) ready = mbar_test_wait(bar_part_full + 8 * part, part_phase);
           } else {
             ptx::tc_fence_before_sync();
             __syncwarp();
@@ -457,26 +491,30 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
 #pragma unroll
       for (int c = 0; c < T::kCols / 32; ++c) {
         const int col0 = n0 + 32 * c;
-        float y[32];
+        uint64_t y[16];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) unpack_f32x2(acc[c * 16 + j], y[2 * j], y[2 * j + 1]);
+        for (int j = 0; j < 16; ++j) y[j] = acc[c * 16 + j];
         if (col0 < g.n) {
-          finish32(y, g, col0);
+          finish32<ACT>(y, g, col0);
           if (p.tma_store) {
             // Row `lane` of the group's 32 x 128-byte buffer, 16-byte chunk i at i ^ (lane & 7): the 128-byte swizzle.
             const uint32_t row_addr = staging + (c >> 1) * kGroupBytes + lane * kRowBytes;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              ptx::st_shared_v4(row_addr + ((((c & 1) * 4 + i) ^ (lane & 7)) << 4), pack_bf16x2(y[8 * i], y[8 * i + 1]),
-                                pack_bf16x2(y[8 * i + 2], y[8 * i + 3]), pack_bf16x2(y[8 * i + 4], y[8 * i + 5]),
-                                pack_bf16x2(y[8 * i + 6], y[8 * i + 7]));
+              ptx::st_shared_v4(row_addr + ((((c & 1) * 4 + i) ^ (lane & 7)) << 4), pack_bf16x2(y[4 * i]), pack_bf16x2(y[4 * i + 1]),
+                                pack_bf16x2(y[4 * i + 2]), pack_bf16x2(y[4 * i + 3]));
             }
           } else {
             // f32 results and rows a tensor map cannot address: turn the 32 x 32 block in shared memory (element c of
             // row r at c ^ r, no bank conflicts either way) and write whole rows, 32 neighbouring elements a store.
             float* block = reinterpret_cast<float*>(smem_raw + (staging - smem_base));
 #pragma unroll
-            for (int j = 0; j < 32; ++j) block[lane * 32 + (j ^ lane)] = y[j];
+            for (int j = 0; j < 16; ++j) {
+              float lo, hi;
+              unpack_f32x2(y[j], lo, hi);
+              block[lane * 32 + ((2 * j) ^ lane)] = lo;
+              block[lane * 32 + ((2 * j + 1) ^ lane)] = hi;
+            }
             __syncwarp();
             const int rows = static_cast<int>(min(static_cast<long long>(32), g.m - (row - lane)));
             if (col0 + lane < g.n) {
@@ -797,7 +835,7 @@ bool make_map(CUtensorMap* map, const void* base, int elem_bytes, long long rows
   return make_tensormap_2d(map, base, elem_bytes, rows, cols, pitch, box_rows, box_cols, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <int BN, int CTAS>
+template <int BN, int CTAS, int ACT>
 int launch(const GemmFp8& g, cudaStream_t stream) {
   using T = Tile<BN, CTAS>;
   CUtensorMap map_a, map_w;
@@ -811,7 +849,7 @@ int launch(const GemmFp8& g, cudaStream_t stream) {
   if (p.tma_store && !make_map(&map_out, g.out, 2, g.m, g.n, g.ldc, 32, 64)) return LC0B200_ERR_CUDA;
   p.status = device_status_words();
   if (p.status == nullptr) return LC0B200_ERR_CUDA;
-  auto kernel = gemm_fp8_kernel<BN, CTAS>;
+  auto kernel = gemm_fp8_kernel<BN, CTAS, ACT>;
   static PerDeviceOnce smem_opt_in;  // per instantiation
   if (allow_dynamic_smem(smem_opt_in, kernel, T::kSmemBytes) != LC0B200_OK) return LC0B200_ERR_CUDA;
   if (T::kSplitRegs) {
@@ -842,6 +880,16 @@ int launch(const GemmFp8& g, cudaStream_t stream) {
     return LC0B200_ERR_CUDA;
   }
   return LC0B200_OK;
+}
+
+template <int BN, int CTAS>
+int launch(const GemmFp8& g, cudaStream_t stream) {
+  switch (g.activation) {
+    case LC0B200_ACT_NONE: return launch<BN, CTAS, LC0B200_ACT_NONE>(g, stream);
+    case LC0B200_ACT_MISH: return launch<BN, CTAS, LC0B200_ACT_MISH>(g, stream);
+    case LC0B200_ACT_RELU: return launch<BN, CTAS, LC0B200_ACT_RELU>(g, stream);
+    default: return launch<BN, CTAS, LC0B200_ACT_SWISH>(g, stream);
+  }
 }
 
 template <int NT>
