@@ -157,28 +157,39 @@ __device__ __forceinline__ int mma_width(int n, int tile_n0) {
   return left >= BN ? BN : ((left + 31) & ~31);
 }
 
-// mish(x) = x n / (n + 2), n = e^x (e^x + 2) (formula: bt4/kernels/layer_norm.py:61-69), of two pairs at a time: packed
-// arithmetic, and one reciprocal for all four (1 / a = b c d / (a b c d)).  The exponential is taken of min(x, 11): there
-// n / (n + 2) rounds to 1, and the product of four denominators stays below 2e38.  What the transcendental unit does is
-// what this costs: five quarter-rate operations for four values instead of eight.
-__device__ __forceinline__ void mish4(uint64_t& xa, uint64_t& xb) {
+// mish(x) = x n / (n + 2), n = e^x (e^x + 2) (formula: bt4/kernels/layer_norm.py:61-69), of PAIRS packed pairs in step: each
+// phase is a run of independent operations.  One reciprocal serves four values (1 / a = b c d / (a b c d)).  The exponential
+// is taken of min(x, 11): there n / (n + 2) rounds to 1, and the product of four denominators stays below 2e38.
+template <int PAIRS>
+__device__ __forceinline__ void mish_pairs(uint64_t* x) {
   const uint64_t two = both_f32x2(2.0f), log2e = both_f32x2(1.4426950408889634f);
-  auto power = [&](uint64_t x) {
-    float lo, hi, elo, ehi;
-    unpack_f32x2(mul_f32x2(x, log2e), lo, hi);
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(elo) : "f"(fminf(lo, 15.8696f)));
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(ehi) : "f"(fminf(hi, 15.8696f)));
-    return pack_f32x2(__float_as_uint(elo), __float_as_uint(ehi));
-  };
-  const uint64_t ea = power(xa), eb = power(xb);
-  const uint64_t na = mul_f32x2(ea, add_f32x2(ea, two)), nb = mul_f32x2(eb, add_f32x2(eb, two));
-  const uint64_t da = add_f32x2(na, two), db = add_f32x2(nb, two);
-  float plo, phi, r;
-  unpack_f32x2(mul_f32x2(da, db), plo, phi);
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(plo * phi));
-  const uint64_t rp = pack_f32x2(__float_as_uint(r * phi), __float_as_uint(r * plo));
-  xa = mul_f32x2(mul_f32x2(xa, na), mul_f32x2(rp, db));
-  xb = mul_f32x2(mul_f32x2(xb, nb), mul_f32x2(rp, da));
+  uint64_t n[PAIRS], d[PAIRS], r[PAIRS / 2];
+#pragma unroll
+  for (int j = 0; j < PAIRS; ++j) {
+    float lo, hi;
+    unpack_f32x2(mul_f32x2(x[j], log2e), lo, hi);
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(lo) : "f"(fminf(lo, 15.8696f)));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(hi) : "f"(fminf(hi, 15.8696f)));
+    n[j] = pack_f32x2(__float_as_uint(lo), __float_as_uint(hi));
+  }
+#pragma unroll
+  for (int j = 0; j < PAIRS; ++j) n[j] = mul_f32x2(n[j], add_f32x2(n[j], two));
+#pragma unroll
+  for (int j = 0; j < PAIRS; ++j) d[j] = add_f32x2(n[j], two);
+#pragma unroll
+  for (int j = 0; j < PAIRS; j += 2) {
+    float lo, hi, inverse;
+    unpack_f32x2(mul_f32x2(d[j], d[j + 1]), lo, hi);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(lo * hi));
+    r[j / 2] = pack_f32x2(__float_as_uint(inverse * hi), __float_as_uint(inverse * lo));
+  }
+#pragma unroll
+  for (int j = 0; j < PAIRS; ++j) x[j] = mul_f32x2(x[j], n[j]);
+#pragma unroll
+  for (int j = 0; j < PAIRS; j += 2) {
+    x[j] = mul_f32x2(x[j], mul_f32x2(r[j / 2], d[j + 1]));
+    x[j + 1] = mul_f32x2(x[j + 1], mul_f32x2(r[j / 2], d[j]));
+  }
 }
 
 // Bias and activation of 32 columns from col0 on, as packed pairs; columns past the matrix edge get no bias (they are not
@@ -205,8 +216,8 @@ __device__ __forceinline__ void finish32(uint64_t (&y)[16], const GemmFp8& g, in
     }
   }
   if (ACT == LC0B200_ACT_MISH) {
-#pragma unroll
-    for (int j = 0; j < 16; j += 2) mish4(y[j], y[j + 1]);
+    mish_pairs<8>(y);
+    mish_pairs<8>(y + 8);
   } else if (ACT != LC0B200_ACT_NONE) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
