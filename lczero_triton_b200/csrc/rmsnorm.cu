@@ -3,7 +3,8 @@
 //   y = v / sqrt(mean(v^2) + eps) * gamma
 //   out = bf16(y), and / or e4m3 codes with a scale per 1 x 128 block of the f32 y (fp8.cuh)
 // Every result is rounded once, from the f32 value: the norm reads v and not the rounded residual, the codes come from
-// y and not from the bf16 row, so that no result depends on which of the others are asked for.
+// y and not from the bf16 row, so that no result depends on which of the others are asked for.  y = (v * gamma) * rstd: the
+// product of two bf16 values is exact, and as rstd is a factor of the whole row, the codes come from v * gamma alone.
 // HBM-bound: a row is read once and kept in registers (rows of more than 16384 channels are read twice).
 #include <cuda_runtime.h>
 
@@ -103,31 +104,57 @@ __global__ void __launch_bounds__(THREADS == 32 ? 32 * kWarpsPerBlock : 256) rms
   }
   sum = row_sum<THREADS>(sum);
   const float rstd = 1.0f / sqrtf(sum / static_cast<float>(p.width) + p.epsilon);
+  if (SKIP && p.residual != nullptr) {
 #pragma unroll
-  for (int g = 0; g < GROUPS; ++g) {
-    if (THREADS * g >= (p.width >> 3)) break;  // the same for every row: the shuffles below have every lane
-    const int idx = t + THREADS * g;
-    const bool here = idx < groups;
-    if (SKIP && p.residual != nullptr && here) reinterpret_cast<uint4*>(p.residual + row * p.ld_residual)[idx] = pack8(v[g]);
-    float gamma[8];
-    unpack8(here ? __ldg(reinterpret_cast<const uint4*>(p.gamma) + idx) : make_uint4(0u, 0u, 0u, 0u), gamma);
+    for (int g = 0; g < GROUPS; ++g) {
+      const int idx = t + THREADS * g;
+      if (idx < groups) reinterpret_cast<uint4*>(p.residual + row * p.ld_residual)[idx] = pack8(v[g]);
+    }
+  }
+  if (rstd == 0.0f) {  // the squares overflowed: zeros, whatever gamma is (an infinity gives NaN)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[g][j] = v[g][j] * rstd * gamma[j];
-    if (p.out != nullptr && here) reinterpret_cast<uint4*>(p.out + row * p.ld_out)[idx] = pack8(v[g]);
+    for (int g = 0; g < GROUPS; ++g) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[g][j] *= 0.0f;
+    }
+  }
+#pragma unroll
+  for (int g0 = 0; g0 < GROUPS; g0 += 4) {
+    if (THREADS * g0 >= (p.width >> 3)) break;  // the same for every row: the shuffles below have every lane
+    uint32_t amax[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int g = g0; g < GROUPS && g < g0 + 4; ++g) {
+      const int idx = t + THREADS * g;
+      if (idx >= groups) continue;
+      float gamma[8], y[8];
+      unpack8(__ldg(reinterpret_cast<const uint4*>(p.gamma) + idx), gamma);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[g][j] *= gamma[j];
+        y[j] = v[g][j] * rstd;
+        if (QUANT) amax[g - g0] = max(amax[g - g0], magnitude_bits(v[g][j]));
+      }
+      if (p.out != nullptr) reinterpret_cast<uint4*>(p.out + row * p.ld_out)[idx] = pack8(y);
+    }
     if (QUANT) {
-      uint32_t amax = 0u;
+      // Sixteen lanes hold block (t + THREADS g) / 16 in step g: four steps at a time, a lane works out one block's scale.
+      float scale, factor;
+      const bool direct = fp8_norm_block_scale(max_of_four_blocks(amax), rstd, scale, factor);
+      const int step = g0 + ((lane >> 2) & 3), block = ((t & ~15) + THREADS * step) / 16;
+      if ((lane & 3) == 0 && step < GROUPS && row < p.rows && block * 16 < groups) p.scale[block * p.ld_scale + row] = scale;
+      const float before = direct ? 1.0f : rstd;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) amax = max(amax, magnitude_bits(v[g][j]));
-      amax = here ? amax : 0u;  // (0 * rstd may be NaN)
+      for (int g = g0; g < GROUPS && g < g0 + 4; ++g) {
+        const int idx = t + THREADS * g;
+        const float f = from_block(factor, g - g0), r = from_block(before, g - g0);
+        if (r != 1.0f) {
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
-      float scale, inverse;
-      fp8_block_scale(amax, scale, inverse);
-      if (here) {
-        if ((lane & 15) == 0) p.scale[(idx >> 4) * p.ld_scale + row] = scale;
-        reinterpret_cast<uint2*>(p.q + row * p.ld_q)[idx] =
-            make_uint2(fp8_pack4(v[g][0] * inverse, v[g][1] * inverse, v[g][2] * inverse, v[g][3] * inverse),
-                       fp8_pack4(v[g][4] * inverse, v[g][5] * inverse, v[g][6] * inverse, v[g][7] * inverse));
+          for (int j = 0; j < 8; ++j) v[g][j] *= r;
+        }
+        if (idx < groups) {
+          reinterpret_cast<uint2*>(p.q + row * p.ld_q)[idx] = make_uint2(fp8_pack4(v[g][0] * f, v[g][1] * f, v[g][2] * f, v[g][3] * f),
+                                                                        fp8_pack4(v[g][4] * f, v[g][5] * f, v[g][6] * f, v[g][7] * f));
+        }
       }
     }
   }
@@ -171,11 +198,15 @@ __device__ __forceinline__ void store_run(const RmsParams& p, long long row, int
       if (FULL || c0 + 32 * i < p.width) residual[32 * i] = __float2bfloat16_rn(v[i]);
     }
   }
+  if (rstd == 0.0f) {  // the squares overflowed: zeros, whatever gamma is (an infinity gives NaN)
+#pragma unroll
+    for (int i = 0; i < CHANNELS; ++i) v[i] *= 0.0f;
+  }
 #pragma unroll
   for (int i = 0; i < CHANNELS; ++i) {
     const bool here = FULL || c0 + 32 * i < p.width;
-    v[i] = here ? v[i] * rstd * __bfloat162float(p.gamma[c0 + 32 * i]) : 0.0f;
-    if (p.out != nullptr && here) out[32 * i] = __float2bfloat16_rn(v[i]);
+    if (here) v[i] *= __bfloat162float(p.gamma[c0 + 32 * i]);  // (zero past the row's end already)
+    if (p.out != nullptr && here) out[32 * i] = __float2bfloat16_rn(v[i] * rstd);
   }
   if (QUANT) {
     uint8_t* q = p.q + row * p.ld_q + c0;
@@ -187,7 +218,10 @@ __device__ __forceinline__ void store_run(const RmsParams& p, long long row, int
 #pragma unroll
       for (int i = b; i < b + 4; ++i) amax = max(amax, magnitude_bits(v[i]));
       float scale, inverse;
-      fp8_block_scale(__reduce_max_sync(0xFFFFFFFFu, amax), scale, inverse);
+      if (!fp8_norm_block_scale(__reduce_max_sync(0xFFFFFFFFu, amax), rstd, scale, inverse)) {
+#pragma unroll
+        for (int i = b; i < b + 4; ++i) v[i] *= rstd;
+      }
       if ((threadIdx.x & 31) == 0) p.scale[block * p.ld_scale + row] = scale;
 #pragma unroll
       for (int i = b; i < b + 4; ++i) {
@@ -255,15 +289,18 @@ __global__ void __launch_bounds__(kThreads) rms_norm_any_kernel(const RmsParams 
       y[j] = 0.0f;
       if (c < p.width) {
         const float v = value(c);
-        y[j] = v * rstd * __bfloat162float(p.gamma[c]);
+        y[j] = (rstd == 0.0f ? v * 0.0f : v) * __bfloat162float(p.gamma[c]);  // (squares that overflow give zeros)
         if (p.residual != nullptr) p.residual[row * p.ld_residual + c] = __float2bfloat16_rn(v);
-        if (p.out != nullptr) p.out[row * p.ld_out + c] = __float2bfloat16_rn(y[j]);
+        if (p.out != nullptr) p.out[row * p.ld_out + c] = __float2bfloat16_rn(y[j] * rstd);
       }
       amax = max(amax, magnitude_bits(y[j]));
     }
     if (p.q != nullptr) {
       float scale, inverse;
-      fp8_block_scale(__reduce_max_sync(0xFFFFFFFFu, amax), scale, inverse);
+      if (!fp8_norm_block_scale(__reduce_max_sync(0xFFFFFFFFu, amax), rstd, scale, inverse)) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] *= rstd;
+      }
       if (lane == 0) p.scale[block * p.ld_scale + row] = scale;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
