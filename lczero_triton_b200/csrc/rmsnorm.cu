@@ -88,6 +88,15 @@ __global__ void __launch_bounds__(THREADS == 32 ? 32 * kWarpsPerBlock : 256) rms
       if (SKIP) raw_skip[g] = skip[idx];
     }
   }
+  // A CTA per row is for few or wide rows, where a second memory round trip shows: gamma comes with the row.
+  constexpr bool kGammaEarly = THREADS == 256 && GROUPS <= 4;
+  uint4 raw_gamma[GROUPS];
+  if (kGammaEarly) {
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+      if (t + THREADS * g < groups) raw_gamma[g] = __ldg(reinterpret_cast<const uint4*>(p.gamma) + t + THREADS * g);
+    }
+  }
   float v[GROUPS][8];
   float sum = 0.0f;
 #pragma unroll
@@ -127,7 +136,7 @@ __global__ void __launch_bounds__(THREADS == 32 ? 32 * kWarpsPerBlock : 256) rms
       const int idx = t + THREADS * g;
       if (idx >= groups) continue;
       float gamma[8], y[8];
-      unpack8(__ldg(reinterpret_cast<const uint4*>(p.gamma) + idx), gamma);
+      unpack8(kGammaEarly ? raw_gamma[g] : __ldg(reinterpret_cast<const uint4*>(p.gamma) + idx), gamma);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         v[g][j] *= gamma[j];
@@ -166,16 +175,17 @@ __global__ void __launch_bounds__(THREADS == 32 ? 32 * kWarpsPerBlock : 256) rms
 // rows took 27 us.  (16-byte or 4-byte words shifted into place move fewer requests and execute three times the instructions.)
 // FULL: the run lies inside the row, nothing is checked per channel.
 template <int CHANNELS, bool SKIP, bool FULL>
-__device__ __forceinline__ float load_run(const RmsParams& p, long long row, int c0, float (&v)[CHANNELS]) {
+__device__ __forceinline__ float load_run(const RmsParams& p, long long row, int c0, float (&v)[CHANNELS], bf16 (&gamma)[CHANNELS]) {
   const bf16* x = p.x + row * p.ld_x + c0;
   const bf16* skip = p.skip + row * p.ld_skip + c0;
   bf16 raw[CHANNELS], raw_skip[CHANNELS];
 #pragma unroll
   for (int i = 0; i < CHANNELS; ++i) {
-    raw[i] = raw_skip[i] = __ushort_as_bfloat16(0);
+    raw[i] = raw_skip[i] = gamma[i] = __ushort_as_bfloat16(0);
     if (FULL || c0 + 32 * i < p.width) {
       raw[i] = x[32 * i];
       if (SKIP) raw_skip[i] = skip[32 * i];
+      gamma[i] = p.gamma[c0 + 32 * i];  // here already: one memory round trip a row, not two
     }
   }
   float sum = 0.0f;
@@ -189,7 +199,7 @@ __device__ __forceinline__ float load_run(const RmsParams& p, long long row, int
 }
 
 template <int CHANNELS, bool SKIP, bool QUANT, bool FULL>
-__device__ __forceinline__ void store_run(const RmsParams& p, long long row, int c0, float (&v)[CHANNELS], float rstd) {
+__device__ __forceinline__ void store_run(const RmsParams& p, long long row, int c0, float (&v)[CHANNELS], const bf16 (&gamma)[CHANNELS], float rstd) {
   bf16* residual = p.residual + row * p.ld_residual + c0;
   bf16* out = p.out + row * p.ld_out + c0;
   if (SKIP && p.residual != nullptr) {
@@ -205,7 +215,7 @@ __device__ __forceinline__ void store_run(const RmsParams& p, long long row, int
 #pragma unroll
   for (int i = 0; i < CHANNELS; ++i) {
     const bool here = FULL || c0 + 32 * i < p.width;
-    if (here) v[i] *= __bfloat162float(p.gamma[c0 + 32 * i]);  // (zero past the row's end already)
+    v[i] *= __bfloat162float(gamma[i]);  // (both zero past the row's end)
     if (p.out != nullptr && here) out[32 * i] = __float2bfloat16_rn(v[i] * rstd);
   }
   if (QUANT) {
@@ -241,15 +251,16 @@ __global__ void __launch_bounds__(1024) rms_norm_odd_kernel(const RmsParams p) {
   const int c0 = 32 * CHANNELS * warp + lane;
   const bool full = 32 * CHANNELS * (warp + 1) <= p.width;
   float v[CHANNELS];
-  float sum = warp_sum(full ? load_run<CHANNELS, SKIP, true>(p, row, c0, v) : load_run<CHANNELS, SKIP, false>(p, row, c0, v));
+  bf16 gamma[CHANNELS];
+  float sum = warp_sum(full ? load_run<CHANNELS, SKIP, true>(p, row, c0, v, gamma) : load_run<CHANNELS, SKIP, false>(p, row, c0, v, gamma));
   if (blockDim.x > 32) {
     if (lane == 0) warp_part[warp] = sum;
     __syncthreads();
     sum = warp_sum(lane < static_cast<int>(blockDim.x >> 5) ? warp_part[lane] : 0.0f);
   }
   const float rstd = 1.0f / sqrtf(sum / static_cast<float>(p.width) + p.epsilon);
-  if (full) store_run<CHANNELS, SKIP, QUANT, true>(p, row, c0, v, rstd);
-  else store_run<CHANNELS, SKIP, QUANT, false>(p, row, c0, v, rstd);
+  if (full) store_run<CHANNELS, SKIP, QUANT, true>(p, row, c0, v, gamma, rstd);
+  else store_run<CHANNELS, SKIP, QUANT, false>(p, row, c0, v, gamma, rstd);
 }
 
 // Any width, pitch and alignment: one CTA per row, the row read twice (the second time from the caches).  Every value
