@@ -58,13 +58,14 @@ __device__ __forceinline__ bool fp8_norm_block_scale(uint32_t amax_bits, float r
   return direct;
 }
 
+__device__ __forceinline__ uint16_t fp8_pack2(float a, float b) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+}
 __device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d) {
   const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
   const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
   return lo | (hi << 16);
 }
-
-__device__ __forceinline__ uint8_t fp8_one(float a) { return __nv_cvt_float_to_fp8(a, __NV_SATFINITE, __NV_E4M3); }
 
 __device__ __forceinline__ float fp8_value(uint8_t code) {
   const __half_raw h = __nv_cvt_fp8_to_halfraw(code, __NV_E4M3);

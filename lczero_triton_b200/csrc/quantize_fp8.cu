@@ -78,17 +78,26 @@ __device__ __forceinline__ void quantize_run(uint8_t* dst, float* scales, long l
       raw[u][i] = FULL || run + at + lane < width ? __ldg(x + at) : 0u;
     }
   }
+  // Lane u works out block u's scale (two divisions once, not UNROLL times).
+  uint32_t mine = 0u;
 #pragma unroll
   for (int u = 0; u < UNROLL; ++u) {
-    if (!FULL && run + kFp8Block * u >= width) break;  // the same for the warp
     const uint32_t m = max(max(raw[u][0] & 0x7FFFu, raw[u][1] & 0x7FFFu), max(raw[u][2] & 0x7FFFu, raw[u][3] & 0x7FFFu));
-    float scale, inverse;
-    fp8_block_scale(__reduce_max_sync(0xFFFFFFFFu, m) << 16, scale, inverse);
-    if (lane == 0) scales[(run / kFp8Block + u) * ld_scale] = scale;
+    const uint32_t block = __reduce_max_sync(0xFFFFFFFFu, m);
+    mine = lane == u ? block : mine;
+  }
+  float scale, inverse;
+  fp8_block_scale(mine << 16, scale, inverse);
+  if (lane < UNROLL && (FULL || run + kFp8Block * lane < width)) scales[(run / kFp8Block + lane) * ld_scale] = scale;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+  for (int u = 0; u < UNROLL; ++u) {
+    const float factor = __shfl_sync(0xFFFFFFFFu, inverse, u);
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
       const int at = kFp8Block * u + 32 * i;
-      if (FULL || run + at + lane < width) q[at] = fp8_one(__uint_as_float(raw[u][i] << 16) * inverse);
+      const uint16_t codes = fp8_pack2(__uint_as_float(raw[u][i] << 16) * factor, __uint_as_float(raw[u][i + 1] << 16) * factor);
+      if (FULL || run + at + lane < width) q[at] = static_cast<uint8_t>(codes);
+      if (FULL || run + at + 32 + lane < width) q[at + 32] = static_cast<uint8_t>(codes >> 8);
     }
   }
 }
@@ -187,11 +196,12 @@ quantize_fp8_odd_tiles_kernel(uint8_t* __restrict__ q_out, float* __restrict__ s
       const long long row = row0 + kWarps * r;
       if (row < rows) {
         uint8_t* dst = q_out + row * ld_out + c0;
-        const float2 a = unpack_bf16x2(raw[r][0]), b = unpack_bf16x2(raw[r][1]);
-        const float v[4] = {a.x, a.y, b.x, b.y};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (c0 + 32 * i < width) dst[32 * i] = fp8_one(v[i] * inverse);
+        for (int i = 0; i < 2; ++i) {
+          const float2 v = unpack_bf16x2(raw[r][i]);
+          const uint16_t codes = fp8_pack2(v.x * inverse, v.y * inverse);
+          if (c0 + 64 * i < width) dst[64 * i] = static_cast<uint8_t>(codes);
+          if (c0 + 64 * i + 32 < width) dst[64 * i + 32] = static_cast<uint8_t>(codes >> 8);
         }
       }
     }

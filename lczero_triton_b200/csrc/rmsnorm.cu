@@ -220,22 +220,28 @@ __device__ __forceinline__ void store_run(const RmsParams& p, long long row, int
   }
   if (QUANT) {
     uint8_t* q = p.q + row * p.ld_q + c0;
+    const int lane = threadIdx.x & 31, block0 = (c0 - lane) / kFp8Block;
+    // Lane u works out block u's scale (three divisions once, not CHANNELS / 4 times).
+    uint32_t mine = 0u;
 #pragma unroll
-    for (int b = 0; b < CHANNELS; b += 4) {
-      const int block = c0 / kFp8Block + b / 4;  // (a lane's first channel is in the run's first block)
-      if (!FULL && block * kFp8Block >= p.width) break;
+    for (int u = 0; u < CHANNELS / 4; ++u) {
       uint32_t amax = 0u;
 #pragma unroll
-      for (int i = b; i < b + 4; ++i) amax = max(amax, magnitude_bits(v[i]));
-      float scale, inverse;
-      if (!fp8_norm_block_scale(__reduce_max_sync(0xFFFFFFFFu, amax), rstd, scale, inverse)) {
+      for (int i = 4 * u; i < 4 * u + 4; ++i) amax = max(amax, magnitude_bits(v[i]));
+      amax = __reduce_max_sync(0xFFFFFFFFu, amax);
+      mine = lane == u ? amax : mine;
+    }
+    float scale, factor;
+    const bool direct = fp8_norm_block_scale(mine, rstd, scale, factor);
+    if (lane < CHANNELS / 4 && (FULL || (block0 + lane) * kFp8Block < p.width)) p.scale[(block0 + lane) * p.ld_scale + row] = scale;
 #pragma unroll
-        for (int i = b; i < b + 4; ++i) v[i] *= rstd;
-      }
-      if ((threadIdx.x & 31) == 0) p.scale[block * p.ld_scale + row] = scale;
+    for (int u = 0; u < CHANNELS / 4; ++u) {
+      const float f = __shfl_sync(0xFFFFFFFFu, factor, u), r = __shfl_sync(0xFFFFFFFFu, direct ? 1.0f : rstd, u);
 #pragma unroll
-      for (int i = b; i < b + 4; ++i) {
-        if (FULL || c0 + 32 * i < p.width) q[32 * i] = fp8_one(v[i] * inverse);
+      for (int i = 4 * u; i < 4 * u + 4; i += 2) {
+        const uint16_t codes = r == 1.0f ? fp8_pack2(v[i] * f, v[i + 1] * f) : fp8_pack2(v[i] * r * f, v[i + 1] * r * f);
+        if (FULL || c0 + 32 * i < p.width) q[32 * i] = static_cast<uint8_t>(codes);
+        if (FULL || c0 + 32 * i + 32 < p.width) q[32 * i + 32] = static_cast<uint8_t>(codes >> 8);
       }
     }
   }
@@ -316,7 +322,7 @@ __global__ void __launch_bounds__(kThreads) rms_norm_any_kernel(const RmsParams 
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int c = block * kFp8Block + 32 * j + lane;
-        if (c < p.width) p.q[row * p.ld_q + c] = fp8_one(y[j] * inverse);
+        if (c < p.width) p.q[row * p.ld_q + c] = static_cast<uint8_t>(fp8_pack2(y[j] * inverse, 0.0f));
       }
     }
   }
