@@ -302,7 +302,8 @@ LC0B200_API int lc0b200_gemm_fp8(void* out, const void* a_e4m3, const float* a_s
                                  long long ld_a_scale, long long ldw, long long ld_w_scale, long long ldc, int out_kind,
                                  int activation, void* stream);
 /* One e4m3 dense layer on bf16 activations: lc0b200_quantize_fp8 (1 x 128 blocks) into caller-provided scratch, then
- * lc0b200_gemm_fp8.  scratch_q holds m * (k rounded up to 16) bytes, scratch_scale m * ceil(k / 128) floats; both 16-byte
+ * lc0b200_gemm_fp8; the same bits in one launch, without the scratch, for at most 16 rows of whole 16-byte words
+ * (k, lda multiples of 8, a 16-byte aligned).  scratch_q holds m * (k rounded up to 16) bytes, scratch_scale m * ceil(k / 128) floats; both 16-byte
  * aligned, reusable as soon as the call's kernels have run (calls that may overlap need scratch of their own). */
 LC0B200_API int lc0b200_linear_fp8(void* out, const void* a_bf16, const void* w_nk_e4m3, const float* w_scale,
                                    const void* bias_bf16, void* scratch_q, float* scratch_scale, long long m, int n, int k,

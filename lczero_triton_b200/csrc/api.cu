@@ -424,6 +424,8 @@ LC0B200_API int lc0b200_linear_fp8(void* out, const void* a, const void* w_nk, c
   int st = check_gemm_fp8(g);
   if (st != LC0B200_OK) return st;
   if (m == 0) return LC0B200_OK;
+  const auto* rows = reinterpret_cast<const bf16*>(a);
+  if (linear_fp8_few_supported(g, rows, lda)) return linear_fp8_few(g, rows, lda, S(stream));
   st = quantize_fp8(scratch_q, scratch_scale, a, m, k, 1, lda, pitch, m, S(stream));
   if (st != LC0B200_OK) return st;
   return gemm_fp8(g, S(stream));

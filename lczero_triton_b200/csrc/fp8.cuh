@@ -67,6 +67,19 @@ __device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d
   return lo | (hi << 16);
 }
 
+// Magnitudes of bf16 values order as 16-bit unsigned integers (NaN above infinity): packed maximum of eight.
+__device__ __forceinline__ uint32_t packed_magnitude(const uint4& raw) {
+  return __vmaxu2(__vmaxu2(raw.x & 0x7FFF7FFFu, raw.y & 0x7FFF7FFFu), __vmaxu2(raw.z & 0x7FFF7FFFu, raw.w & 0x7FFF7FFFu));
+}
+// The larger half of a packed maximum as float bits.
+__device__ __forceinline__ uint32_t magnitude_of_packed(uint32_t m) { return max(m & 0xFFFFu, m >> 16) << 16; }
+
+__device__ __forceinline__ uint2 codes8(const uint4& raw, float inverse) {
+  const float2 a = unpack_bf16x2(raw.x), b = unpack_bf16x2(raw.y), c = unpack_bf16x2(raw.z), d = unpack_bf16x2(raw.w);
+  return make_uint2(fp8_pack4(a.x * inverse, a.y * inverse, b.x * inverse, b.y * inverse),
+                    fp8_pack4(c.x * inverse, c.y * inverse, d.x * inverse, d.y * inverse));
+}
+
 __device__ __forceinline__ float fp8_value(uint8_t code) {
   const __half_raw h = __nv_cvt_fp8_to_halfraw(code, __NV_E4M3);
   return __half2float(__half(h));

@@ -148,6 +148,8 @@ struct FpParams {
   GemmFp8 g;
   int tma_store;  // bf16 result with a base, pitch and width that a tensor map can store
   unsigned int* status;
+  const bf16* a_bf16;  // few-row kernel on bf16 rows: they are quantised on the way in (g.a, g.a_scale are not read)
+  long long ld_a_bf16;
 };
 
 // Columns that the MMAs of the tile at tile_n0 cover: a ragged last tile costs its own width rounded up to 32.
@@ -612,7 +614,11 @@ __device__ __forceinline__ void store_one(float y, const GemmFp8& g, long long a
   else reinterpret_cast<bf16*>(g.out)[at] = __float2bfloat16_rn(y);
 }
 
-template <int NT>
+// BF16_A: the dense layer on bf16 rows in one launch.  The scale warps bring the tokens' rows of a k block, apply the
+// block rule of quantize_fp8 (the same bits) and write the codes where the tensor map would have put them.  Every weight
+// tile does this again for its tokens, from the L2: worth it for the few tokens of one MMA column group (two launches
+// for 8 tokens, 8192 x 2048: 9.2 us on the GPU and 12.6 us a call).
+template <int NT, bool BF16_A>
 __global__ void __launch_bounds__(Few<NT>::kThreads, 2)
 gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const FpParams p) {
   using T = Few<NT>;
@@ -656,7 +662,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
   if (threadIdx.x == 0) {
     *abort_flag = aligned ? 0 : 1;
     for (int s = 0; s < kStages; ++s) {
-      ptx::mbar_init(bar_full + 8 * s, 1);
+      ptx::mbar_init(bar_full + 8 * s, BF16_A ? 2 : 1);  // the copies, and the warp that writes the codes
       ptx::mbar_init(bar_empty + 8 * s, 1);
     }
     for (int a = 0; a < kPartials; ++a) {
@@ -665,7 +671,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     }
     ptx::mbar_init_fence();
     ptx::prefetch_tensormap(&map_w);
-    ptx::prefetch_tensormap(&map_a);
+    if (!BF16_A) ptx::prefetch_tensormap(&map_a);
   }
   if (warp == 1) {
     ptx::tmem_alloc(tmem_slot, T::kTmemCols);
@@ -688,10 +694,11 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
       ok = __all_sync(0xFFFFFFFFu, ok);
       if (!ok) break;
       if (ptx::elect_one()) {
-        ptx::mbar_expect_tx(bar_full + 8 * stage, T::kStageBytes);
+        ptx::mbar_expect_tx(bar_full + 8 * stage, BF16_A ? T::kWBytes : T::kStageBytes);
         ptx::tma_load_2d<1>(smem_w + stage * T::kWBytes, &map_w, kb * kFp8Block, n0, bar_full + 8 * stage);
-        ptx::tma_load_2d<1>(smem_a + stage * NT * kRowBytes, &map_a, kb * kFp8Block, static_cast<int>(m0),
-                            bar_full + 8 * stage);
+        if (!BF16_A) {
+          ptx::tma_load_2d<1>(smem_a + stage * NT * kRowBytes, &map_a, kb * kFp8Block, static_cast<int>(m0), bar_full + 8 * stage);
+        }
       }
       if (++stage == kStages) {
         stage = 0;
@@ -736,17 +743,64 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     uint32_t phase = 0;
     for (int kb = kb_begin + first; kb < kb_end && ok; kb += 2) {
       const float w = __ldg(w_scale + kb);
-      const float* a_scale = g.a_scale + kb * g.ld_a_scale + m0;
-      const float a0 = lane < tokens ? __ldg(a_scale + lane) : 0.0f;
-      const float a1 = NT > 32 && lane + 32 < tokens ? __ldg(a_scale + lane + 32) : 0.0f;
-      ok = ptx::mbar_wait(bar_part_empty + 8 * part, phase ^ 1u, abort_flag, p.status, 0x2500u + part);
-      ok = __all_sync(0xFFFFFFFFu, ok);
-      if (!ok) break;
-      const uint32_t dst = scale_base + part * T::kScaleBytes + lane * 4;
-      if (lane < NT) asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst), "f"(a0 * w) : "memory");
-      if (NT > 32) asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst + 128), "f"(a1 * w) : "memory");
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(bar_part_full + 8 * part);
+      if constexpr (BF16_A) {
+        // A half-warp holds a token's block in step i: tokens 2 i and 2 i + 1.
+        constexpr int kSteps = NT / 2;
+        static_assert(kSteps % 4 == 0, "scales are worked out four steps at a time");
+        const int lane16 = lane & 15, side = lane >> 4;
+        const int channel = kb * kFp8Block + lane16 * 8;
+        uint4 raw[kSteps];
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+          const bool here = 2 * i + side < tokens && channel < g.k;
+          raw[i] = here ? __ldg(reinterpret_cast<const uint4*>(p.a_bf16 + (m0 + 2 * i + side) * p.ld_a_bf16 + channel)) : make_uint4(0u, 0u, 0u, 0u);
+        }
+        const int at = kb - kb_begin, stage = at % kStages;
+        ok = ptx::mbar_wait(bar_part_empty + 8 * part, phase ^ 1u, abort_flag, p.status, 0x2500u + part) &&
+             ptx::mbar_wait(bar_empty + 8 * stage, ((at / kStages) & 1u) ^ 1u, abort_flag, p.status, 0x2600u + stage);
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        if (!ok) break;
+#pragma unroll
+        for (int i0 = 0; i0 < kSteps; i0 += 4) {
+          uint32_t m[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) m[i] = magnitude_of_packed(packed_magnitude(raw[i0 + i]));
+          float scale, inverse;
+          fp8_block_scale(max_of_four_blocks(m), scale, inverse);
+          if ((lane & 3) == 0) {
+            const int token = 2 * (i0 + (lane16 >> 2)) + side;
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(scale_base + part * T::kScaleBytes + token * 4), "f"(scale * w) : "memory");
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            // Row `token` of the stage's 128-byte swizzled tile: 16-byte chunk c lies at c ^ (token & 7).
+            const int token = 2 * (i0 + i) + side;
+            const uint2 codes = codes8(raw[i0 + i], from_block(inverse, i));
+            asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(smem_a + stage * NT * kRowBytes + token * kRowBytes +
+                                                                (((lane16 >> 1) ^ (token & 7)) << 4) + (lane16 & 1) * 8),
+                         "r"(codes.x), "r"(codes.y)
+                         : "memory");
+          }
+        }
+        ptx::fence_proxy_async_smem();  // the MMAs read the codes through the asynchronous proxy
+        __syncwarp();
+        if (lane == 0) {
+          ptx::mbar_arrive(bar_full + 8 * stage);
+          ptx::mbar_arrive(bar_part_full + 8 * part);
+        }
+      } else {
+        const float* a_scale = g.a_scale + kb * g.ld_a_scale + m0;
+        const float a0 = lane < tokens ? __ldg(a_scale + lane) : 0.0f;
+        const float a1 = NT > 32 && lane + 32 < tokens ? __ldg(a_scale + lane + 32) : 0.0f;
+        ok = ptx::mbar_wait(bar_part_empty + 8 * part, phase ^ 1u, abort_flag, p.status, 0x2500u + part);
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        if (!ok) break;
+        const uint32_t dst = scale_base + part * T::kScaleBytes + lane * 4;
+        if (lane < NT) asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst), "f"(a0 * w) : "memory");
+        if (NT > 32) asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst + 128), "f"(a1 * w) : "memory");
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(bar_part_full + 8 * part);
+      }
       part += 2;
       if (part >= kPartials) {
         part = first;
@@ -855,6 +909,8 @@ int launch(const GemmFp8& g, cudaStream_t stream) {
   FpParams p;
   p.g = g;
   // (A TMA store clips a row at whole 16 bytes: with n not a multiple of 8 it would write into the pitch.)
+  p.a_bf16 = nullptr;
+  p.ld_a_bf16 = 0;
   p.tma_store = g.out_kind == LC0B200_OUT_BF16 && aligned16(g.out) && (g.ldc % 8) == 0 && (g.n % 8) == 0;
   CUtensorMap map_out = map_a;  // placeholder when unused
   if (p.tma_store && !make_map(&map_out, g.out, 2, g.m, g.n, g.ldc, 32, 64)) return LC0B200_ERR_CUDA;
@@ -903,18 +959,21 @@ int launch(const GemmFp8& g, cudaStream_t stream) {
   }
 }
 
-template <int NT>
-int launch_few(const GemmFp8& g, cudaStream_t stream) {
+template <int NT, bool BF16_A = false>
+int launch_few(const GemmFp8& g, cudaStream_t stream, const bf16* a_bf16 = nullptr, long long ld_a_bf16 = 0) {
   using T = Few<NT>;
   CUtensorMap map_a, map_w;
   if (!make_map(&map_w, g.w, 1, g.n, g.k, g.ldw, kBM, kFp8Block)) return LC0B200_ERR_CUDA;
-  if (!make_map(&map_a, g.a, 1, g.m, g.k, g.lda, NT, kFp8Block)) return LC0B200_ERR_CUDA;
+  map_a = map_w;  // placeholder when unused
+  if (!BF16_A && !make_map(&map_a, g.a, 1, g.m, g.k, g.lda, NT, kFp8Block)) return LC0B200_ERR_CUDA;
   FpParams p;
   p.g = g;
   p.tma_store = 0;
+  p.a_bf16 = a_bf16;
+  p.ld_a_bf16 = ld_a_bf16;
   p.status = device_status_words();
   if (p.status == nullptr) return LC0B200_ERR_CUDA;
-  auto kernel = gemm_fp8_few_kernel<NT>;
+  auto kernel = gemm_fp8_few_kernel<NT, BF16_A>;
   static PerDeviceOnce smem_opt_in;  // per instantiation
   if (allow_dynamic_smem(smem_opt_in, kernel, T::kSmemBytes) != LC0B200_OK) return LC0B200_ERR_CUDA;
   // Split k while every CTA stays resident, two to an SM, and has a k block at least.
@@ -944,6 +1003,16 @@ int launch_few(const GemmFp8& g, cudaStream_t stream) {
 }
 
 }  // namespace
+
+bool linear_fp8_few_supported(const GemmFp8& g, const bf16* a, long long lda) {
+  return g.m <= 16 && (g.k % 8) == 0 && aligned16(a) && (lda % 8 == 0 || g.m == 1) && aligned16(g.w) && (g.ldw % 16 == 0 || g.n == 1);
+}
+
+int linear_fp8_few(const GemmFp8& given, const bf16* a, long long lda, cudaStream_t stream) {
+  GemmFp8 g = given;
+  if (g.n == 1) g.ldw = ceil_div_ll(g.k, 16) * 16;
+  return launch_few<16, true>(g, stream, a, lda);
+}
 
 int gemm_fp8(const GemmFp8& given, cudaStream_t stream) {
   GemmFp8 g = given;

@@ -23,6 +23,9 @@ struct GemmFp8 {
 
 // Chooses the kernel by what the operands allow.
 int gemm_fp8(const GemmFp8& g, cudaStream_t stream);
+// The dense layer on few bf16 rows in one launch (g.a, g.a_scale, g.lda and g.ld_a_scale are not used).
+bool linear_fp8_few_supported(const GemmFp8& g, const bf16* a, long long lda);
+int linear_fp8_few(const GemmFp8& g, const bf16* a, long long lda, cudaStream_t stream);
 // CUDA-core kernel: any pitch and alignment.
 int gemm_fp8_simt(const GemmFp8& g, cudaStream_t stream);
 

@@ -14,19 +14,6 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kRowsPerCta = kThreads / 16;  // a half-warp (16 lanes x 8 values) holds one 1 x 128 block
 
-// Magnitudes of bf16 values order as 16-bit unsigned integers (NaN above infinity): packed maximum of eight.
-__device__ __forceinline__ uint32_t packed_magnitude(const uint4& raw) {
-  return __vmaxu2(__vmaxu2(raw.x & 0x7FFF7FFFu, raw.y & 0x7FFF7FFFu), __vmaxu2(raw.z & 0x7FFF7FFFu, raw.w & 0x7FFF7FFFu));
-}
-// The larger half of a packed maximum as float bits.
-__device__ __forceinline__ uint32_t magnitude_of_packed(uint32_t m) { return max(m & 0xFFFFu, m >> 16) << 16; }
-
-__device__ __forceinline__ uint2 codes8(const uint4& raw, float inverse) {
-  const float2 a = unpack_bf16x2(raw.x), b = unpack_bf16x2(raw.y), c = unpack_bf16x2(raw.z), d = unpack_bf16x2(raw.w);
-  return make_uint2(fp8_pack4(a.x * inverse, a.y * inverse, b.x * inverse, b.y * inverse),
-                    fp8_pack4(c.x * inverse, c.y * inverse, d.x * inverse, d.y * inverse));
-}
-
 // Rows of whole, aligned 16-byte words: a half-warp takes four neighbouring blocks of one row, a CTA 16 rows.  (With every
 // lane reducing and dividing for all four blocks the kernel was bound by its instructions: 262144 x 1536 in 203 us.)
 __global__ void __launch_bounds__(kThreads)

@@ -395,7 +395,7 @@ def linear_fp8(out: torch.Tensor, a: torch.Tensor, w: torch.Tensor, w_scale: tor
         return out
     check(_lib.load().lc0b200_linear_fp8(_p(out), _p(a), _p(w), _p(w_scale), _p(bias), _p(scratch_q), _p(scratch_scale),
                                          m, n, k, lda, ldw, ld_w_scale, ldc, kind,
-                                         ACTIVATIONS[activation], _raw_stream(device)), "linear_fp8", launches=2)
+                                         ACTIVATIONS[activation], _raw_stream(device)), "linear_fp8", launches=1 if m <= 16 else 2)
     return out
 
 

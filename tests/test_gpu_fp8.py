@@ -432,6 +432,33 @@ def test_linear(ops, m, n, k) -> None:
         _untouched(out)
 
 
+@pytest.mark.parametrize("m", [1, 2, 7, 8, 15, 16, 17])
+@pytest.mark.parametrize("n, k, extra", [(256, 512, 0), (1000, 1000, 8), (129, 136, 24), (4096, 2048, 0), (40, 8, 0)])
+def test_linear_few_rows(ops, m, n, k, extra) -> None:
+    """Up to 16 rows run as one launch: still the bits of its two parts, also where blocks are zeros, tiny or not finite."""
+    x = _pitched(m, k, BF16, k + extra, 8 if extra else 0)
+    x.copy_(_rows(43, m, k))
+    x[0, : min(k, 128)] = 0.0
+    if m > 2:
+        x[1] *= 2.0 ** -125
+        x[2, k // 2] = float("nan")
+    if m > 7:
+        x[5, k - 1] = float("-inf")
+        x[6, :4] = torch.finfo(BF16).max
+    _, _, w, w_scale = _operands(44, 1, n, k)
+    w = _placed(w, -(-k // 16) * 16)
+    bias = torch.randn(n, generator=_gen(45)).to(BF16).cuda()
+    q, scale = _pitched(m, k, FP8, -(-k // 16) * 16), torch.empty((-(-k // 128), m), device="cuda")
+    ops.quantize_fp8(q, scale, x)
+    for dtype, activation in ((BF16, "none"), (torch.float32, "mish")):
+        want, out = torch.empty((m, n), dtype=dtype, device="cuda"), _pitched(m, n, dtype, n + 3)
+        ops.gemm_fp8(want, q, scale, w, w_scale, bias=bias, activation=activation)
+        ops.linear_fp8(out, x, w, w_scale, bias, *_scratch(m, k), activation=activation)
+        assert torch.equal(torch.isnan(out), torch.isnan(want))
+        assert torch.equal(torch.nan_to_num(out, nan=0.0), torch.nan_to_num(want, nan=0.0))
+        _untouched(out)
+
+
 def _block(ops, s) -> None:
     """A feed-forward block as a decoder runs it: norm of the residual straight to codes, two products, next norm."""
     ops.rms_norm(None, s["x"], s["gamma1"], skip=s["residual"], residual_out=s["residual1"], q_out=s["q"], q_scale=s["q_scale"])
