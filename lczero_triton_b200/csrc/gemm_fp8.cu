@@ -358,20 +358,18 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         for (int kb = 0; kb < k_blocks; ++kb) {
           // The operands first: they are there early, and the look at their barrier is off the path from a freed partial.
           ok = ptx::mbar_wait(bar_full + 8 * stage, phase, abort_flag, p.status, 0x1300u + stage);
+          const uint64_t a_desc = ptx::smem_desc_sw128(smem_a + stage * T::kABytes, 16, 1024);
+          const uint64_t b_desc = ptx::smem_desc_sw128(smem_b + stage * T::kBBytes, 16, 1024);
           ok = ok && ptx::mbar_wait(bar_part_empty + 8 * part, part_phase ^ 1u, abort_flag, p.status, 0x1200u + part);
-          ok = __all_sync(0xFFFFFFFFu, ok);
           if (!ok) break;
           ptx::tc_fence_after_sync();
           if (ptx::elect_one()) {
-            const uint32_t a_addr = smem_a + stage * T::kABytes;
-            const uint32_t b_addr = smem_b + stage * T::kBBytes;
 #pragma unroll
             for (int j = 0; j < kFp8Block / kMmaK; ++j) {
-              mma_e4m3<CTAS>(tmem_base + part * BN, ptx::smem_desc_sw128(a_addr + j * kMmaK, 16, 1024),
-                             ptx::smem_desc_sw128(b_addr + j * kMmaK, 16, 1024), idesc, j > 0 ? 1u : 0u);
+              mma_e4m3<CTAS>(tmem_base + part * BN, a_desc + j * (kMmaK >> 4), b_desc + j * (kMmaK >> 4), idesc, j > 0 ? 1u : 0u);
             }
-            ptx::tc_commit<CTAS>(bar_empty + 8 * stage);
             ptx::tc_commit<CTAS>(bar_part_full + 8 * part);
+            ptx::tc_commit<CTAS>(bar_empty + 8 * stage);
           }
           if (++stage == kStages) {
             stage = 0;
