@@ -1,6 +1,7 @@
 // CUDA-core form of the block-scaled e4m3 product, for operands TMA cannot address (a base or a row pitch that is not a
 // multiple of 16 bytes) and as an independent cross-check of the tensor-core kernels.  64 x 64 output tile per CTA,
-// 4 x 4 per thread; codes are scaled to f32 as they enter shared memory.
+// 4 x 4 per thread, bound by the fp32 pipes and shared memory.  As in them, a block's sum is formed from the codes and then
+// multiplied by the product of its two scales.
 #include <cuda_runtime.h>
 
 #include "common.cuh"
@@ -13,7 +14,7 @@ namespace {
 
 constexpr int kTile = 64;
 constexpr int kTileK = 16;
-static_assert(kFp8Block % kTileK == 0, "a step along k must not straddle two scales");
+static_assert(kFp8Block % kTileK == 0 && kFp8Block % kTile == 0, "a step along k, or a tile, must not straddle two scales");
 
 __global__ void __launch_bounds__(256) gemm_fp8_simt_kernel(const GemmFp8 p) {
   grid_dependency_release();
@@ -23,15 +24,14 @@ __global__ void __launch_bounds__(256) gemm_fp8_simt_kernel(const GemmFp8 p) {
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const long long m0 = static_cast<long long>(blockIdx.x) * kTile;
   const int n0 = blockIdx.y * kTile;
-  float acc[4][4] = {};
+  float acc[4][4] = {}, block[4][4] = {};
   for (int k0 = 0; k0 < p.k; k0 += kTileK) {
-    const int kb = k0 / kFp8Block;
     for (int i = threadIdx.x; i < kTile * kTileK; i += 256) {
       const int r = i / kTileK, c = i % kTileK;
       const long long gm = m0 + r;
       const int gn = n0 + r, gk = k0 + c;
-      sa[c][r] = (gm < p.m && gk < p.k) ? fp8_value(p.a[gm * p.lda + gk]) * p.a_scale[kb * p.ld_a_scale + gm] : 0.0f;
-      sw[c][r] = (gn < p.n && gk < p.k) ? fp8_value(p.w[gn * p.ldw + gk]) * p.w_scale[(gn / kFp8Block) * p.ld_w_scale + kb] : 0.0f;
+      sa[c][r] = (gm < p.m && gk < p.k) ? fp8_value(p.a[gm * p.lda + gk]) : 0.0f;
+      sw[c][r] = (gn < p.n && gk < p.k) ? fp8_value(p.w[gn * p.ldw + gk]) : 0.0f;
     }
     __syncthreads();
 #pragma unroll
@@ -44,7 +44,21 @@ __global__ void __launch_bounds__(256) gemm_fp8_simt_kernel(const GemmFp8 p) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(av[i], wv[j], acc[i][j]);
+        for (int j = 0; j < 4; ++j) block[i][j] = fmaf(av[i], wv[j], block[i][j]);
+      }
+    }
+    if (k0 + kTileK >= p.k || (k0 + kTileK) % kFp8Block == 0) {
+      const int kb = k0 / kFp8Block;
+      const float w_scale = p.w_scale[(n0 / kFp8Block) * p.ld_w_scale + kb];  // a tile lies in one row of scales
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const long long gm = m0 + ty * 4 + i;
+        const float scale = gm < p.m ? p.a_scale[kb * p.ld_a_scale + gm] * w_scale : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          acc[i][j] = fmaf(block[i][j], scale, acc[i][j]);
+          block[i][j] = 0.0f;
+        }
       }
     }
     __syncthreads();

@@ -398,6 +398,48 @@ def test_gemm_extreme_scales(ops) -> None:
         _close(out, want[:rows], size[:rows], k)
 
 
+@pytest.mark.parametrize("m, pitch", [(5, 256), (5, 257), (200, 257)])
+def test_gemm_scales_that_only_fit_together(ops, m, pitch) -> None:
+    """Scale times code overflows, the product of the two scales does not."""
+    n, k = 130, 256
+    a, a_scale, w, w_scale = _operands(34, m, n, k)
+    a_scale *= 2.0 ** 126
+    w_scale *= 2.0 ** -126
+    want, size = F8.gemm(a, a_scale, w, w_scale)
+    out = torch.empty((m, n), device="cuda")
+    ops.gemm_fp8(out, _placed(a, pitch), a_scale, _placed(w, pitch), w_scale)
+    _close(out, want, size, k)
+
+
+@pytest.mark.parametrize("m, n", [(3, 300), (200, 300)])
+def test_offsets_past_32_bits(ops, m, n) -> None:
+    """Rows and scales a long way apart: every operand's last row begins past element 2^31."""
+    k, far = 384, (2 ** 31 // (m - 1) // 64 + 1) * 64
+    def apart(rows, columns, dtype, pitch):
+        return torch.empty((rows - 1) * pitch + columns, dtype=dtype, device="cuda").as_strided((rows, columns), (pitch, 1))
+    x = apart(m, k, BF16, far)
+    x.copy_(_rows(35, m, k))
+    q, scale = apart(m, k, FP8, far), apart(3, m, torch.float32, 2 ** 30 + 4)
+    ops.quantize_fp8(q, scale, x)
+    codes, want_scale = F8.quantize(x)
+    _same_codes(q, codes)
+    _same_floats(scale, want_scale)
+    w = torch.randn((n, k), generator=_gen(36)).to(BF16).cuda()
+    w_q, w_scale = torch.empty((n, k), dtype=FP8, device="cuda"), torch.empty((-(-n // 128), 3), device="cuda")
+    ops.quantize_fp8(w_q, w_scale, w, block_rows=128)
+    want, size = F8.gemm(q, scale, w_q, w_scale)
+    out = apart(m, n, BF16, far)
+    ops.gemm_fp8(out, q, scale, w_q, w_scale)
+    _close(out, want, size, k)
+    out.zero_()
+    ops.linear_fp8(out, x, w_q, w_scale, None, *_scratch(m, k))
+    _close(out, want, size, k)
+    gamma = torch.ones(k, dtype=BF16, device="cuda")
+    norm = apart(m, k, BF16, far)
+    ops.rms_norm(norm, x, gamma, epsilon=1e-6, q_out=q, q_scale=scale)
+    _check_norm(x, None, gamma, 1e-6, norm, None, q, scale)
+
+
 def test_no_rows(ops) -> None:
     a, a_scale, w, w_scale = _operands(31, 4, 64, 128)
     ops.gemm_fp8(torch.empty((0, 64), dtype=BF16, device="cuda"), a[:0], a_scale[:, :0], w, w_scale)
