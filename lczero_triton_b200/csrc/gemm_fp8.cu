@@ -161,7 +161,8 @@ __device__ __forceinline__ int mma_width(int n, int tile_n0) {
 
 // mish(x) = x n / (n + 2), n = e^x (e^x + 2) (formula: bt4/kernels/layer_norm.py:61-69), of PAIRS packed pairs in step: each
 // phase is a run of independent operations.  One reciprocal serves four values (1 / a = b c d / (a b c d)).  The exponential
-// is taken of min(x, 11): there n / (n + 2) rounds to 1, and the product of four denominators stays below 2e38.
+// is taken of min(x, 10): there n / (n + 2) rounds to 1, and the product of four denominators stays below 6e34, so that its
+// reciprocal is far from the values that the fast reciprocal flushes to zero.
 template <int PAIRS>
 __device__ __forceinline__ void mish_pairs(uint64_t* x) {
   const uint64_t two = both_f32x2(2.0f), log2e = both_f32x2(1.4426950408889634f);
@@ -170,8 +171,8 @@ __device__ __forceinline__ void mish_pairs(uint64_t* x) {
   for (int j = 0; j < PAIRS; ++j) {
     float lo, hi;
     unpack_f32x2(mul_f32x2(x[j], log2e), lo, hi);
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(lo) : "f"(fminf(lo, 15.8696f)));
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(hi) : "f"(fminf(hi, 15.8696f)));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(lo) : "f"(fminf(lo, 14.42695f)));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(hi) : "f"(fminf(hi, 14.42695f)));
     n[j] = pack_f32x2(__float_as_uint(lo), __float_as_uint(hi));
   }
 #pragma unroll
@@ -186,11 +187,9 @@ __device__ __forceinline__ void mish_pairs(uint64_t* x) {
     r[j / 2] = pack_f32x2(__float_as_uint(inverse * hi), __float_as_uint(inverse * lo));
   }
 #pragma unroll
-  for (int j = 0; j < PAIRS; ++j) x[j] = mul_f32x2(x[j], n[j]);
-#pragma unroll
-  for (int j = 0; j < PAIRS; j += 2) {
-    x[j] = mul_f32x2(x[j], mul_f32x2(r[j / 2], d[j + 1]));
-    x[j + 1] = mul_f32x2(x[j + 1], mul_f32x2(r[j / 2], d[j]));
+  for (int j = 0; j < PAIRS; j += 2) {  // n / (n + 2) first: x n may overflow
+    x[j] = mul_f32x2(x[j], mul_f32x2(n[j], mul_f32x2(r[j / 2], d[j + 1])));
+    x[j + 1] = mul_f32x2(x[j + 1], mul_f32x2(n[j + 1], mul_f32x2(r[j / 2], d[j])));
   }
 }
 
@@ -603,8 +602,7 @@ struct Few {
 
 __device__ __forceinline__ float finish_one(float y, const GemmFp8& g, int column) {
   if (g.bias != nullptr) y += __bfloat162float(g.bias[column]);
-  if (g.activation == LC0B200_ACT_RELU) return y < 0.0f ? 0.0f : y;  // NaN stays
-  return activate_rt(y, g.activation);
+  return fp8_activate(y, g.activation);
 }
 
 __device__ __forceinline__ void store_one(float y, const GemmFp8& g, long long at) {

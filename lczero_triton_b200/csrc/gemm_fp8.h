@@ -21,6 +21,13 @@ struct GemmFp8 {
   int out_kind, activation;
 };
 
+// One value's activation.  A NaN stays one, and so does an infinity (mish(y) rounds to y above 20).
+__device__ __forceinline__ float fp8_activate(float y, int activation) {
+  if (activation == LC0B200_ACT_RELU) return y < 0.0f ? 0.0f : y;
+  if (activation == LC0B200_ACT_MISH && y > 20.0f) return y;
+  return activate_rt(y, activation);
+}
+
 // Chooses the kernel by what the operands allow.
 int gemm_fp8(const GemmFp8& g, cudaStream_t stream);
 // The dense layer on few bf16 rows in one launch (g.a, g.a_scale, g.lda and g.ld_a_scale are not used).

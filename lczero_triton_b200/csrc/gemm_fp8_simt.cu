@@ -72,8 +72,7 @@ __global__ void __launch_bounds__(256) gemm_fp8_simt_kernel(const GemmFp8 p) {
       const int gn = n0 + tx * 4 + j;
       if (gn >= p.n) continue;
       float y = acc[i][j] + (p.bias != nullptr ? __bfloat162float(p.bias[gn]) : 0.0f);
-      if (p.activation == LC0B200_ACT_RELU) y = y < 0.0f ? 0.0f : y;  // NaN stays
-      else y = activate_rt(y, p.activation);
+      y = fp8_activate(y, p.activation);
       if (p.out_kind == LC0B200_OUT_F32) reinterpret_cast<float*>(p.out)[gm * p.ldc + gn] = y;
       else reinterpret_cast<bf16*>(p.out)[gm * p.ldc + gn] = __float2bfloat16_rn(y);
     }

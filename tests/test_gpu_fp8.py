@@ -320,6 +320,34 @@ def test_gemm_activations(ops, activation, m, n, k) -> None:
         _close(out, want, size, k, activation)
 
 
+# Few rows, then both tile shapes, each with the CUDA-core form beside it (an odd pitch).
+@pytest.mark.parametrize("activation", ["mish", "relu", "swish"])
+@pytest.mark.parametrize("m, pitch", [(3, 128), (70, 128), (70, 129), (4000, 128), (6000, 128)])
+def test_gemm_activation_range(ops, activation, m, pitch) -> None:
+    """Neighbouring columns that are all small, all large or infinite: codes of zero, so that the sum is the bias."""
+    n, k = 520, 128
+    a, w = (_placed(torch.zeros((rows, k), device="cuda").to(FP8), pitch) for rows in (m, n))
+    a_scale, w_scale = torch.ones((1, m), device="cuda"), torch.ones((5, 1), device="cuda")
+    bias = torch.linspace(-60.0, 60.0, n).to(BF16)
+    bias[-8:] = torch.tensor([1e4, 1e10, 1e19, 1e30, 3e38, 1e5, 80.0, float("inf")]).to(BF16)
+    bias = bias.cuda()
+    want = F8.activate(bias.double(), activation)
+    want[-1] = float("inf")
+    for dtype in (BF16, torch.float32):
+        out = torch.empty((m, n), dtype=dtype, device="cuda")
+        ops.gemm_fp8(out, a, a_scale, w, w_scale, bias=bias, activation=activation)
+        assert bool((out[:, -1] == float("inf")).all())
+        error = (out[:, :-1].double() - want[:-1]).abs()
+        allowed = want[:-1].abs() * ((2.0 ** -8 if dtype is BF16 else U) + 1e-5)
+        assert bool((error <= allowed).all()), float((error - allowed).max())
+
+
+@pytest.mark.parametrize("activation", ["mish", "relu", "swish"])
+@pytest.mark.parametrize("m, n", [(4000, 520), (6000, 1000)])
+def test_gemm_activations_of_large_tiles(ops, activation, m, n) -> None:
+    test_gemm_activations(ops, activation, m, n, 384)
+
+
 # Large enough for every tile shape and several tiles per CTA.
 @pytest.mark.parametrize("m, n, k", [(1, 4096, 4096), (8, 8192, 2048), (16, 1024, 8192), (48, 1536, 1024), (64, 24576, 256),
                                      (96, 4096, 1024), (777, 1858, 1000), (2048, 1024, 1024), (4096, 1536, 512),
