@@ -275,9 +275,9 @@ LC0B200_API int lc0b200_linear_int8_static(void* out_bf16, const void* a_bf16, c
  *   saturated.  A block with an infinity or a NaN gets a non-finite scale and reads back as NaN throughout.
  * The last block of a row (and the last rows of a matrix) may be short.  Scales of activations are block-major like the
  * row statistics of lc0b200_gemm: scale[block * ld_scale + row], ld_scale >= rows; scales of weights are
- * scale[(row / 128) * ld_scale + column / 128].  All ld* are row pitches in elements.  Outputs may not overlap inputs
- * except where said.  Bytes between a row's width and its pitch are never
- * written; they may be read, and are ignored. */
+ * scale[(row / 128) * ld_scale + column / 128].  All ld* are row pitches in elements.  Outputs may overlap neither each
+ * other nor, except where said, inputs.  Bytes between a row's width and its pitch are never written; they may be read,
+ * and are ignored. */
 
 /* bf16 rows to codes; block_rows is 1 (activations) or 128 (weights, at load time).  Any alignment; 16-byte aligned
  * input rows and 8-byte aligned output rows are the fast form. */
@@ -287,7 +287,8 @@ LC0B200_API int lc0b200_quantize_fp8(void* out_e4m3, float* scale_f32, const voi
  * y = v / sqrt(mean(v^2) + epsilon) * gamma, fp32; out = bf16(y) and / or q_out, q_scale = block rule on y (each pair may
  * be NULL, not both).  Every output is rounded once from its fp32 value.  out and residual_out may be in or skip
  * themselves (same pointer and pitch).  A pitch belongs to its pointer and is ignored where that is NULL.
- * A row whose mean square overflows fp32 (values above about 1e19) gives zeros. */
+ * v * gamma is formed first and the sum of squares is fp32: y is wanted where both are finite fp32 numbers.  A row of
+ * finite values whose sum of squares overflows (values above 1e19 / sqrt(width) or so) gives zeros. */
 LC0B200_API int lc0b200_rms_norm(void* out_bf16, void* residual_out_bf16, void* q_out_e4m3, float* q_scale_f32,
                                  const void* in_bf16, const void* skip_bf16, const void* gamma_bf16, long long row_count,
                                  int width, float epsilon, long long ld_in, long long ld_skip, long long ld_out,
@@ -303,8 +304,9 @@ LC0B200_API int lc0b200_gemm_fp8(void* out, const void* a_e4m3, const float* a_s
                                  int activation, void* stream);
 /* One e4m3 dense layer on bf16 activations: lc0b200_quantize_fp8 (1 x 128 blocks) into caller-provided scratch, then
  * lc0b200_gemm_fp8; the same bits in one launch, without the scratch, for at most 16 rows of whole 16-byte words
- * (k, lda multiples of 8, a 16-byte aligned).  scratch_q holds m * (k rounded up to 16) bytes, scratch_scale m * ceil(k / 128) floats; both 16-byte
- * aligned, reusable as soon as the call's kernels have run (calls that may overlap need scratch of their own). */
+ * (k, lda multiples of 8, a 16-byte aligned) and a weight that runs on the tensor cores.  scratch_q holds
+ * m * (k rounded up to 16) bytes, scratch_scale m * ceil(k / 128) floats; both 16-byte aligned, reusable as soon as the
+ * call's kernels have run (calls that may overlap need scratch of their own). */
 LC0B200_API int lc0b200_linear_fp8(void* out, const void* a_bf16, const void* w_nk_e4m3, const float* w_scale,
                                    const void* bias_bf16, void* scratch_q, float* scratch_scale, long long m, int n, int k,
                                    long long lda, long long ldw, long long ld_w_scale, long long ldc, int out_kind,

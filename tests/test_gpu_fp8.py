@@ -237,6 +237,33 @@ def test_rms_norm_special_rows(ops, width) -> None:
     assert bool(torch.isnan(out[0]).all())  # 0 / 0
 
 
+@pytest.mark.parametrize("width", [64, 256, 1024, 1111, 4096, 9001, 17000])
+@pytest.mark.parametrize("of_x, of_gamma, epsilon", [(-50, -40, 0.0), (-60, 0, 1e-6), (-60, -70, 1e-6), (50, 60, 0.0), (60, -100, 1e-6)])
+def test_rms_norm_far_from_one(ops, width, of_x, of_gamma, epsilon) -> None:
+    """Rows and gammas of small and large powers of two (their products are fp32 numbers), blocks that count as zeros, rows
+    whose sum of squares is past fp32."""
+    rows = 200
+    x, skip = _rows(13, rows, width) * 2.0 ** of_x, _rows(14, rows, width) * 2.0 ** of_x
+    gamma = ((1 + 0.2 * torch.randn(width, generator=_gen(15))) * 2.0 ** of_gamma).to(BF16).cuda()
+    for n in (3, rows):
+        out, q = torch.empty((n, width), dtype=BF16, device="cuda"), torch.empty((n, width), dtype=FP8, device="cuda")
+        scale = torch.empty((-(-width // 128), n), device="cuda")
+        ops.rms_norm(out, x[:n], gamma, epsilon=epsilon, skip=skip[:n], q_out=q, q_scale=scale)
+        squares = (x[:n].double() + skip[:n].double()).square().sum(dim=1)
+        fits, lost = squares < 0.99 * 2.0 ** 128, squares > 1.01 * 2.0 ** 128
+        assert of_x >= 60 or bool(fits.all())
+        _check_norm(x[:n][fits], skip[:n][fits], gamma, epsilon, out[fits], None, q[fits], scale[:, fits])
+        assert bool((out[lost] == 0).all()) and bool((q[lost].float() == 0).all()) and bool((scale[:, lost] == 1).all())
+
+
+@pytest.mark.parametrize("width", [64, 1024, 1111, 20000])
+def test_rms_norm_of_a_row_added_to_itself(ops, width) -> None:
+    x, gamma = _rows(16, 5, width), torch.ones(width, dtype=BF16, device="cuda")
+    before, residual = x.clone(), torch.empty_like(x)
+    ops.rms_norm(x, x, gamma, skip=x, residual_out=residual)
+    _check_norm(before, before, gamma, 1e-6, x, residual, None, None)
+
+
 # ------------------------------------------------------------------ product
 
 def _operands(seed: int, m: int, n: int, k: int):
