@@ -111,6 +111,17 @@ __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_add
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
+// After a wait that ran out: the loads under way still write into this CTA's memory.  Waits for the last one of every stage,
+// a millisecond at the most; `stage` and `phase` are where the next load would have gone.
+__device__ __forceinline__ void drain_loads(uint32_t bar_full, int stages, int stage, uint32_t phase) {
+  const uint64_t start = ptx::globaltimer_ns();
+  for (int s = 0; s < stages; ++s) {
+    const uint32_t parity = s < stage ? phase : phase ^ 1u;
+    while (!ptx::mbar_try_wait(bar_full + 8 * s, parity) && ptx::globaltimer_ns() - start < 1000000u) {
+    }
+  }
+}
+
 template <int BN, int CTAS>
 struct Tile {
   static_assert(CTAS == 1 || (CTAS == 2 && BN == 256), "CTA pairs share 256 x 256 tiles");
@@ -343,6 +354,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         }
       }
     }
+    if (!ok && rank == 0) drain_loads(bar_full, kStages, stage, phase);
     __syncwarp();
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMAs (leader CTA only): one partial per k block
@@ -701,6 +713,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         phase ^= 1u;
       }
     }
+    if (!ok) drain_loads(bar_full, kStages, stage, phase);
     __syncwarp();
   } else if (warp == 1) {
     constexpr uint32_t idesc = ptx::instr_desc(1u, 0u, 0u, kBM, NT);
@@ -816,6 +829,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     uint32_t part_phase = 0;
     for (int kb = kb_begin; kb < kb_end && ok; ++kb) {
       ok = ptx::mbar_wait(bar_part_full + 8 * part, part_phase, abort_flag, p.status, 0x2400u + part);
+      ok = __all_sync(0xFFFFFFFFu, ok);
       if (!ok) break;
       ptx::tc_fence_after_sync();
       uint32_t v[T::kCols];
