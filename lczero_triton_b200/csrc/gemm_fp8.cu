@@ -328,119 +328,120 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
 
   if (warp < 4) {
     if (T::kSplitRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(T::kFrontRegs));
-  if (warp == 0) {
-    // ------------------------------------------------------------ loads: the warp follows the loop, one lane issues
-    int stage = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    for (long long tile = group; tile < num_tiles && ok; tile += num_groups) {
-      const int m0 = static_cast<int>(tile / n_tiles) * kTileM + static_cast<int>(rank) * kBM;
-      const int tile_n0 = static_cast<int>(tile % n_tiles) * BN;
-      // A pair splits the weight tile's rows between its CTAs.
-      const int n0 = tile_n0 + static_cast<int>(rank) * (mma_width<BN>(g.n, tile_n0) / CTAS);
-      for (int kb = 0; kb < k_blocks; ++kb) {
-        ok = ptx::mbar_wait(bar_empty + 8 * stage, phase ^ 1u, abort_flag, p.status, 0x1100u + stage);
-        ok = __all_sync(0xFFFFFFFFu, ok);
-        if (!ok) break;
-        if (ptx::elect_one()) {
-          const uint32_t full = (CTAS == 2) ? ptx::map_to_cta(bar_full + 8 * stage, 0u) : bar_full + 8 * stage;
-          if (rank == 0) ptx::mbar_expect_tx(bar_full + 8 * stage, T::kStageBytes * CTAS);
-          ptx::tma_load_2d<CTAS>(smem_a + stage * T::kABytes, &map_a, kb * kFp8Block, m0, full);
-          ptx::tma_load_2d<CTAS>(smem_b + stage * T::kBBytes, &map_w, kb * kFp8Block, n0, full);
-        }
-        if (++stage == kStages) {
-          stage = 0;
-          phase ^= 1u;
-        }
-      }
-    }
-    if (!ok && rank == 0) drain_loads(bar_full, kStages, stage, phase);
-    __syncwarp();
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMAs (leader CTA only): one partial per k block
-    if (rank == 0) {
-      int stage = 0, part = 0;
-      uint32_t phase = 0, part_phase = 0;
+    if (warp == 0) {
+      // ------------------------------------------------------------ loads: the warp follows the loop, one lane issues
+      int stage = 0;
+      uint32_t phase = 0;
       bool ok = true;
       for (long long tile = group; tile < num_tiles && ok; tile += num_groups) {
+        const int m0 = static_cast<int>(tile / n_tiles) * kTileM + static_cast<int>(rank) * kBM;
         const int tile_n0 = static_cast<int>(tile % n_tiles) * BN;
-        const uint32_t idesc = ptx::instr_desc(1u, 0u, 0u, static_cast<uint32_t>(kTileM),
-                                               static_cast<uint32_t>(mma_width<BN>(g.n, tile_n0)));
+        // A pair splits the weight tile's rows between its CTAs.
+        const int n0 = tile_n0 + static_cast<int>(rank) * (mma_width<BN>(g.n, tile_n0) / CTAS);
         for (int kb = 0; kb < k_blocks; ++kb) {
-          // The operands first: they are there early, and the look at their barrier is off the path from a freed partial.
-          ok = ptx::mbar_wait(bar_full + 8 * stage, phase, abort_flag, p.status, 0x1300u + stage);
-          const uint64_t a_desc = ptx::smem_desc_sw128(smem_a + stage * T::kABytes, 16, 1024);
-          const uint64_t b_desc = ptx::smem_desc_sw128(smem_b + stage * T::kBBytes, 16, 1024);
-          ok = ok && ptx::mbar_wait(bar_part_empty + 8 * part, part_phase ^ 1u, abort_flag, p.status, 0x1200u + part);
+          ok = ptx::mbar_wait(bar_empty + 8 * stage, phase ^ 1u, abort_flag, p.status, 0x1100u + stage);
+          ok = __all_sync(0xFFFFFFFFu, ok);
           if (!ok) break;
-          ptx::tc_fence_after_sync();
           if (ptx::elect_one()) {
-#pragma unroll
-            for (int j = 0; j < kFp8Block / kMmaK; ++j) {
-              mma_e4m3<CTAS>(tmem_base + part * BN, a_desc + j * (kMmaK >> 4), b_desc + j * (kMmaK >> 4), idesc, j > 0 ? 1u : 0u);
-            }
-            ptx::tc_commit<CTAS>(bar_part_full + 8 * part);
-            ptx::tc_commit<CTAS>(bar_empty + 8 * stage);
+            const uint32_t full = (CTAS == 2) ? ptx::map_to_cta(bar_full + 8 * stage, 0u) : bar_full + 8 * stage;
+            if (rank == 0) ptx::mbar_expect_tx(bar_full + 8 * stage, T::kStageBytes * CTAS);
+            ptx::tma_load_2d<CTAS>(smem_a + stage * T::kABytes, &map_a, kb * kFp8Block, m0, full);
+            ptx::tma_load_2d<CTAS>(smem_b + stage * T::kBBytes, &map_w, kb * kFp8Block, n0, full);
           }
           if (++stage == kStages) {
             stage = 0;
             phase ^= 1u;
           }
-          if (++part == kPartials) {
-            part = 0;
-            part_phase ^= 1u;
+        }
+      }
+      if (!ok && rank == 0) drain_loads(bar_full, kStages, stage, phase);
+      __syncwarp();
+    } else if (warp == 1) {
+      // ------------------------------------------------------------ MMAs (leader CTA only): one partial per k block
+      if (rank == 0) {
+        int stage = 0, part = 0;
+        uint32_t phase = 0, part_phase = 0;
+        bool ok = true;
+        for (long long tile = group; tile < num_tiles && ok; tile += num_groups) {
+          const int tile_n0 = static_cast<int>(tile % n_tiles) * BN;
+          const uint32_t idesc = ptx::instr_desc(1u, 0u, 0u, static_cast<uint32_t>(kTileM),
+                                                 static_cast<uint32_t>(mma_width<BN>(g.n, tile_n0)));
+          for (int kb = 0; kb < k_blocks; ++kb) {
+            // The operands first: they are there early, and the look at their barrier is off the path from a freed partial.
+            ok = ptx::mbar_wait(bar_full + 8 * stage, phase, abort_flag, p.status, 0x1300u + stage);
+            const uint64_t a_desc = ptx::smem_desc_sw128(smem_a + stage * T::kABytes, 16, 1024);
+            const uint64_t b_desc = ptx::smem_desc_sw128(smem_b + stage * T::kBBytes, 16, 1024);
+            ok = ok && ptx::mbar_wait(bar_part_empty + 8 * part, part_phase ^ 1u, abort_flag, p.status, 0x1200u + part);
+            if (!ok) break;
+            ptx::tc_fence_after_sync();
+            if (ptx::elect_one()) {
+#pragma unroll
+              for (int j = 0; j < kFp8Block / kMmaK; ++j) {
+                mma_e4m3<CTAS>(tmem_base + part * BN, a_desc + j * (kMmaK >> 4), b_desc + j * (kMmaK >> 4), idesc, j > 0 ? 1u : 0u);
+              }
+              ptx::tc_commit<CTAS>(bar_part_full + 8 * part);
+              ptx::tc_commit<CTAS>(bar_empty + 8 * stage);
+            }
+            if (++stage == kStages) {
+              stage = 0;
+              phase ^= 1u;
+            }
+            if (++part == kPartials) {
+              part = 0;
+              part_phase ^= 1u;
+            }
           }
         }
       }
-    }
-    __syncwarp();
-  } else {
-    // ------------------------------------------------------------ scales: a_scale[row] * w_scale of each k block
-    // Two warps take the k blocks in turn; the scales of a block wait in shared memory beside its partial, behind the
-    // same barrier.  (Epilogue warps that fetched their own were slower, 176 us against 137 at 32768 x 1024 x 4096 in the
-    // worst schedule: a wait for tensor memory may then also wait for a global load.)
-    const int first = warp - 2;
-    int part = first;
-    uint32_t phase = 0;
-    long long tile = group;
-    int kb = first;
-    while (true) {
-      while (kb >= k_blocks) {
-        kb -= k_blocks;
-        tile += num_groups;
-      }
-      if (tile >= num_tiles) break;
-      const long long row0 = (tile / n_tiles) * kTileM + rank * kBM + lane;
-      const int column = static_cast<int>(tile % n_tiles) * BN;
-      float a[4], w[T::kScaleCols];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] = row0 + 32 * i < g.m ? __ldg(g.a_scale + kb * g.ld_a_scale + row0 + 32 * i) : 0.0f;
-#pragma unroll
-      for (int h = 0; h < T::kScaleCols; ++h) {
-        const int n0 = column + h * kFp8Block;
-        w[h] = n0 < g.n ? __ldg(g.w_scale + (n0 / kFp8Block) * g.ld_w_scale + kb) : 0.0f;
-      }
-      bool ok = ptx::mbar_wait(bar_scale_empty + 8 * part, phase ^ 1u, abort_flag, p.status, 0x1500u + part);
-      ok = __all_sync(0xFFFFFFFFu, ok);
-      if (!ok) break;
-#pragma unroll
-      for (int h = 0; h < T::kScaleCols; ++h) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          asm volatile("st.shared.f32 [%0], %1;" ::"r"(scale_base + part * T::kScaleBytes + (h * kBM + 32 * i + lane) * 4), "f"(a[i] * w[h]) : "memory");
+      __syncwarp();
+    } else {
+      // ------------------------------------------------------------ scales: a_scale[row] * w_scale of each k block
+      // Two warps take the k blocks in turn; the scales of a block wait in shared memory beside its partial, behind the
+      // same barrier.  (Epilogue warps that fetched their own were slower, 176 us against 137 at 32768 x 1024 x 4096 in the
+      // worst schedule: a wait for tensor memory may then also wait for a global load.)
+      const int first = warp - 2;
+      int part = first;
+      uint32_t phase = 0;
+      long long tile = group;
+      int kb = first;
+      while (true) {
+        while (kb >= k_blocks) {
+          kb -= k_blocks;
+          tile += num_groups;
         }
+        if (tile >= num_tiles) break;
+        const long long row0 = (tile / n_tiles) * kTileM + rank * kBM + lane;
+        const int column = static_cast<int>(tile % n_tiles) * BN;
+        float a[4], w[T::kScaleCols];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = row0 + 32 * i < g.m ? __ldg(g.a_scale + kb * g.ld_a_scale + row0 + 32 * i) : 0.0f;
+#pragma unroll
+        for (int h = 0; h < T::kScaleCols; ++h) {
+          const int n0 = column + h * kFp8Block;
+          w[h] = n0 < g.n ? __ldg(g.w_scale + (n0 / kFp8Block) * g.ld_w_scale + kb) : 0.0f;
+        }
+        bool ok = ptx::mbar_wait(bar_scale_empty + 8 * part, phase ^ 1u, abort_flag, p.status, 0x1500u + part);
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        if (!ok) break;
+#pragma unroll
+        for (int h = 0; h < T::kScaleCols; ++h) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t at = scale_base + part * T::kScaleBytes + (h * kBM + 32 * i + lane) * 4;
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(a[i] * w[h]) : "memory");
+          }
+        }
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(bar_part_full + 8 * part);
+        part += 2;
+        if (part >= kPartials) {
+          part = first;
+          phase ^= 1u;
+        }
+        kb += 2;
       }
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(bar_part_full + 8 * part);
-      part += 2;
-      if (part >= kPartials) {
-        part = first;
-        phase ^= 1u;
-      }
-      kb += 2;
     }
-    __syncwarp();
-  }
   } else {
     if (T::kSplitRegs) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(T::kEpilogueRegs));
     // ------------------------------------------------------------ epilogue: scale and sum the partials, then store
@@ -918,9 +919,9 @@ int launch(const GemmFp8& g, cudaStream_t stream) {
   if (!make_map(&map_w, g.w, 1, g.n, g.k, g.ldw, T::kBRows, kFp8Block)) return LC0B200_ERR_CUDA;
   FpParams p;
   p.g = g;
-  // (A TMA store clips a row at whole 16 bytes: with n not a multiple of 8 it would write into the pitch.)
   p.a_bf16 = nullptr;
   p.ld_a_bf16 = 0;
+  // (A TMA store clips a row at whole 16 bytes: with n not a multiple of 8 it would write into the pitch.)
   p.tma_store = g.out_kind == LC0B200_OUT_BF16 && aligned16(g.out) && (g.ldc % 8) == 0 && (g.n % 8) == 0;
   CUtensorMap map_out = map_a;  // placeholder when unused
   if (p.tma_store && !make_map(&map_out, g.out, 2, g.m, g.n, g.ldc, 32, 64)) return LC0B200_ERR_CUDA;
@@ -933,7 +934,9 @@ int launch(const GemmFp8& g, cudaStream_t stream) {
     // A register split that asks for more than the launch has would wait for ever.
     static const int launch_regs = [](auto k) {
       cudaFuncAttributes attributes;
-      return cudaFuncGetAttributes(&attributes, k) == cudaSuccess ? attributes.numRegs : 0;
+      if (cudaFuncGetAttributes(&attributes, k) == cudaSuccess) return attributes.numRegs;
+      (void)cudaGetLastError();
+      return 0;
     }(kernel);
     if (launch_regs < T::kLaunchRegs) return LC0B200_ERR_UNSUPPORTED;
   }
