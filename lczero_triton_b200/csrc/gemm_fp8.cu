@@ -12,6 +12,8 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "fp8.cuh"
 #include "gemm_fp8.h"
@@ -253,6 +255,22 @@ __device__ __forceinline__ uint32_t pack_bf16x2(uint64_t pair) {
   return lc0b200::pack_bf16x2(lo, hi);
 }
 
+// The tiles of a CTA (pair), every num_groups-th: row and column of the tile without a division each.
+struct TileWalk {
+  long long tile, m;
+  int n;
+  __device__ TileWalk(long long first, int n_tiles) : tile(first), m(first / n_tiles), n(static_cast<int>(first % n_tiles)) {}
+  __device__ void next(uint32_t groups, int step_m, int step_n, int n_tiles) {
+    tile += groups;
+    m += step_m;
+    n += step_n;
+    if (n >= n_tiles) {
+      n -= n_tiles;
+      ++m;
+    }
+  }
+};
+
 template <int BN, int CTAS, int ACT>
 __global__ void __launch_bounds__(Tile<BN, CTAS>::kThreads, 1)
 gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
@@ -292,6 +310,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
   const int n_tiles = (g.n + BN - 1) / BN;
   const long long num_tiles = ceil_div_ll(g.m, kTileM) * n_tiles;
   const int k_blocks = (g.k + kFp8Block - 1) / kFp8Block;
+  const int step_m = static_cast<int>(num_groups) / n_tiles, step_n = static_cast<int>(num_groups) % n_tiles;
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
@@ -402,16 +421,16 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       const int first = warp - 2;
       int part = first;
       uint32_t phase = 0;
-      long long tile = group;
+      TileWalk walk(group, n_tiles);
       int kb = first;
       while (true) {
         while (kb >= k_blocks) {
           kb -= k_blocks;
-          tile += num_groups;
+          walk.next(num_groups, step_m, step_n, n_tiles);
         }
-        if (tile >= num_tiles) break;
-        const long long row0 = (tile / n_tiles) * kTileM + rank * kBM + lane;
-        const int column = static_cast<int>(tile % n_tiles) * BN;
+        if (walk.tile >= num_tiles) break;
+        const long long row0 = walk.m * kTileM + rank * kBM + lane;
+        const int column = walk.n * BN;
         float a[4], w[T::kScaleCols];
 #pragma unroll
         for (int i = 0; i < 4; ++i) a[i] = row0 + 32 * i < g.m ? __ldg(g.a_scale + kb * g.ld_a_scale + row0 + 32 * i) : 0.0f;
@@ -453,118 +472,179 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     int part = 0;
     uint32_t part_phase = 0;
     bool ok = true;
-    auto row_of = [&](long long tile) { return (tile / n_tiles) * kTileM + rank * kBM + quarter * 32 + lane; };
-    auto column_of = [&](long long tile) { return static_cast<int>(tile % n_tiles) * BN + half * T::kCols; };
     const uint32_t my_scale = scale_base + ((half * T::kCols / kFp8Block) * kBM + quarter * 32 + lane) * 4;
-    for (long long tile = group; tile < num_tiles && ok; tile += num_groups) {
-      const long long row = row_of(tile);
-      const int n0 = column_of(tile);
-      // Running sums as packed pairs of fp32: one packed multiply-add for two columns.
-      constexpr int kChunks = T::kCols / 32;
-      static_assert(kChunks % 2 == 0, "a block's first columns go to the first buffer");
-      uint64_t acc[T::kCols / 2];
+    // Running sums as packed pairs of fp32: one packed multiply-add for two columns.
+    constexpr int kChunks = T::kCols / 32;
+    static_assert(kChunks % 2 == 0, "a block's first columns go to the first buffer");
+    uint64_t acc[T::kCols / 2];
+    float scale = 0.0f;
+    // Waits for the next partial and fetches its scale.
+    auto begin_block = [&](float& block_scale) {
+      ok = ptx::mbar_wait(bar_part_full + 8 * part, part_phase, abort_flag, p.status, 0x1400u + part);
+      if (!ok) return;
+      ptx::tc_fence_after_sync();
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(block_scale) : "r"(my_scale + part * T::kScaleBytes) : "memory");
+    };
+    // Hands a partial that has been read back to the MMAs, its scales back to their warps.
+    auto end_block = [&](int which) {
+      ptx::tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) {
+        if (CTAS == 2) mbar_arrive_cluster_relaxed(ptx::map_to_cta(bar_part_empty + 8 * which, 0u));
+        else ptx::mbar_arrive(bar_part_empty + 8 * which);
+        ptx::mbar_arrive(bar_scale_empty + 8 * which);
+      }
+    };
+    auto take_part = [&]() {
+      const int taken = part;
+      if (++part == kPartials) {
+        part = 0;
+        part_phase ^= 1u;
+      }
+      return taken;
+    };
+    constexpr bool kOverlap = CTAS == 2;  // tiles of one CTA are for problems of about one tile each
+    constexpr int kTaken = kOverlap ? 1 : 0;
+    long long row = 0;  // of the tile whose sums are being formed or finished
+    int n0 = 0;
+    // Stores the 32 columns from col0 on, chunk c of the tile; `tma`: into the staging buffers of a tensor map's store.
+    auto store_chunk = [&](int c, int col0, uint64_t (&y)[16], bool tma) {
+      if (tma) {
+        // Row `lane` of the group's 32 x 128-byte buffer, 16-byte chunk i at i ^ (lane & 7): the 128-byte swizzle.
+        const uint32_t row_addr = staging + (c >> 1) * kGroupBytes + lane * kRowBytes;
 #pragma unroll
-      for (int i = 0; i < T::kCols / 2; ++i) acc[i] = 0ull;
+        for (int i = 0; i < 4; ++i) {
+          ptx::st_shared_v4(row_addr + ((((c & 1) * 4 + i) ^ (lane & 7)) << 4), pack_bf16x2(y[4 * i]),
+                            pack_bf16x2(y[4 * i + 1]), pack_bf16x2(y[4 * i + 2]), pack_bf16x2(y[4 * i + 3]));
+        }
+        return;
+      }
+      // f32 results and rows a tensor map cannot address: turn the 32 x 32 block in shared memory (element c of
+      // row r at c ^ r, no bank conflicts either way) and write whole rows, 32 neighbouring elements a store, eight rows in
+      // flight (20000 x 1858 x 1024 with mish: 106 us, 130 row by row).
+      float* block = reinterpret_cast<float*>(smem_raw + (staging - smem_base));
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        float lo, hi;
+        unpack_f32x2(y[j], lo, hi);
+        block[lane * 32 + ((2 * j) ^ lane)] = lo;
+        block[lane * 32 + ((2 * j + 1) ^ lane)] = hi;
+      }
+      __syncwarp();
+      const int rows = static_cast<int>(min(static_cast<long long>(32), g.m - (row - lane)));
+      if (col0 + lane < g.n) {
+        const long long at = (row - lane) * g.ldc + col0 + lane;
+        if (g.out_kind == LC0B200_OUT_F32) {
+          float* dst = reinterpret_cast<float*>(g.out) + at;
+#pragma unroll 8
+          for (int r = 0; r < rows; ++r) dst[r * g.ldc] = block[r * 32 + (lane ^ r)];
+        } else {
+          bf16* dst = reinterpret_cast<bf16*>(g.out) + at;
+#pragma unroll 8
+          for (int r = 0; r < rows; ++r) dst[r * g.ldc] = __float2bfloat16_rn(block[r * 32 + (lane ^ r)]);
+        }
+      }
+      __syncwarp();
+    };
+
+    // After a tile's last block.  FINISH: bias, activation and store, 32 columns at a time.  TAKE: the next tile's first block
+    // into registers that are free; with both, what finishing frees, so that its columns are on their way while the stores
+    // are issued and the MMAs get the partial back earlier (only for results a tensor map stores, which issue quickly).
+    // 262144 x 1536 x 1024 with mish: 611 us with one after the other, 580 so.
+    auto turn = [&](auto finish, auto take) {
+      constexpr bool kFinish = decltype(finish)::value, kTake = decltype(take)::value;
+      if (kTake) begin_block(scale);
+      if (kTake && !ok) return;
+      const int this_part = kTake ? take_part() : 0;
+      uint64_t scale2 = 0ull;
+      uint32_t w[32];
+      if (kFinish && (kTake || p.tma_store)) {
+        if (lane == 0) ptx::bulk_wait_read<0>();  // the staging buffers are free once the last tile's stores have read them
+        __syncwarp();
+      }
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        const int col0 = n0 + 32 * c;
+        uint64_t y[16];
+        if (kFinish && (kTake || col0 < g.n)) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) y[j] = acc[c * 16 + j];
+          finish32<ACT>(y, g, col0);
+          if (kTake) ptx::tmem_ld_32x32(tmem_row + this_part * BN + 32 * c, w);
+          store_chunk(c, col0, y, kTake || p.tma_store);
+        } else if (kTake) {
+          ptx::tmem_ld_32x32(tmem_row + this_part * BN + 32 * c, w);
+        }
+        if (kTake) {
+          tmem_wait(w);
+          if (c == 0) scale2 = both_f32x2(scale);
+          if (c + 1 == kChunks) end_block(this_part);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) acc[c * 16 + j] = mul_f32x2(pack_f32x2(w[2 * j], w[2 * j + 1]), scale2);
+        }
+      }
+      // After the partial is back with the MMAs: this takes 650 cycles.
+      if (kFinish && (kTake || p.tma_store)) {
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+#pragma unroll
+          for (int i = 0; i < T::kGroups; ++i) {
+            if (n0 + 64 * i < g.n) ptx::tma_store_2d(&map_out, staging + i * kGroupBytes, n0 + 64 * i, static_cast<int>(row));
+          }
+          ptx::bulk_commit();
+        }
+      }
+    };
+
+    using Yes = std::true_type;
+    using No = std::false_type;
+    TileWalk walk(group, n_tiles);
+    bool fresh = true;  // no block of the tile has been taken
+    while (walk.tile < num_tiles && ok) {
+      if (kOverlap && fresh) turn(No{}, Yes{});
+      if (!ok) break;
+      row = walk.m * kTileM + rank * kBM + quarter * 32 + lane;
+      n0 = walk.n * BN + half * T::kCols;
       // 32 columns at a time: while they are added, the next 32 are on their way, across the k blocks too (a partial is
       // handed back, and the next one's first columns asked for, before the last additions).  Columns past the matrix
       // edge hold anything and are not stored.
-      float scale = 0.0f, next_scale = 0.0f;
+      if (!kOverlap) {
+#pragma unroll
+        for (int i = 0; i < T::kCols / 2; ++i) acc[i] = 0ull;
+      }
       uint32_t v[2][32];
-      auto begin_block = [&](float& block_scale) {
-        ok = ptx::mbar_wait(bar_part_full + 8 * part, part_phase, abort_flag, p.status, 0x1400u + part);
-        if (!ok) return;
-        ptx::tc_fence_after_sync();
+      if (k_blocks > kTaken) {
+        begin_block(scale);
         ptx::tmem_ld_32x32(tmem_row + part * BN, v[0]);
-        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(block_scale) : "r"(my_scale + part * T::kScaleBytes) : "memory");
-      };
-      begin_block(scale);
-      for (int kb = 0; kb < k_blocks && ok; ++kb) {
-        const uint64_t scale2 = pack_f32x2(__float_as_uint(scale), __float_as_uint(scale));
-        const int this_part = part;
-        if (++part == kPartials) {
-          part = 0;
-          part_phase ^= 1u;
-        }
+      }
+      for (int kb = kTaken; kb < k_blocks && ok; ++kb) {
+        const uint64_t scale2 = both_f32x2(scale);
+        const int this_part = take_part();
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
           tmem_wait(v[c & 1]);
           if (c + 1 < kChunks) {
             ptx::tmem_ld_32x32(tmem_row + this_part * BN + 32 * (c + 1), v[(c + 1) & 1]);
           } else {
-            ptx::tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) {
-              if (CTAS == 2) mbar_arrive_cluster_relaxed(ptx::map_to_cta(bar_part_empty + 8 * this_part, 0u));
-              else ptx::mbar_arrive(bar_part_empty + 8 * this_part);
-              ptx::mbar_arrive(bar_scale_empty + 8 * this_part);
+            end_block(this_part);
+            if (kb + 1 < k_blocks) {
+              begin_block(scale);
+              ptx::tmem_ld_32x32(tmem_row + part * BN, v[0]);
             }
-            if (kb + 1 < k_blocks) begin_block(next_scale);
           }
 #pragma unroll
           for (int j = 0; j < 16; ++j) fma_f32x2(acc[c * 16 + j], pack_f32x2(v[c & 1][2 * j], v[c & 1][2 * j + 1]), scale2);
         }
-        scale = next_scale;
       }
-      if (!ok) break;
-      // ---- bias, activation, store
-      if (p.tma_store) {
-        if (lane == 0) ptx::bulk_wait_read<0>();  // the staging buffers are free once the last tile's stores have read them
-        __syncwarp();
+      if (!ok) {
+        tmem_wait(v[0]);  // asked for all the same, and not to arrive in registers that hold something else
+        break;
       }
-#pragma unroll
-      for (int c = 0; c < T::kCols / 32; ++c) {
-        const int col0 = n0 + 32 * c;
-        uint64_t y[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) y[j] = acc[c * 16 + j];
-        if (col0 < g.n) {
-          finish32<ACT>(y, g, col0);
-          if (p.tma_store) {
-            // Row `lane` of the group's 32 x 128-byte buffer, 16-byte chunk i at i ^ (lane & 7): the 128-byte swizzle.
-            const uint32_t row_addr = staging + (c >> 1) * kGroupBytes + lane * kRowBytes;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              ptx::st_shared_v4(row_addr + ((((c & 1) * 4 + i) ^ (lane & 7)) << 4), pack_bf16x2(y[4 * i]), pack_bf16x2(y[4 * i + 1]),
-                                pack_bf16x2(y[4 * i + 2]), pack_bf16x2(y[4 * i + 3]));
-            }
-          } else {
-            // f32 results and rows a tensor map cannot address: turn the 32 x 32 block in shared memory (element c of
-            // row r at c ^ r, no bank conflicts either way) and write whole rows, 32 neighbouring elements a store.
-            float* block = reinterpret_cast<float*>(smem_raw + (staging - smem_base));
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              float lo, hi;
-              unpack_f32x2(y[j], lo, hi);
-              block[lane * 32 + ((2 * j) ^ lane)] = lo;
-              block[lane * 32 + ((2 * j + 1) ^ lane)] = hi;
-            }
-            __syncwarp();
-            const int rows = static_cast<int>(min(static_cast<long long>(32), g.m - (row - lane)));
-            if (col0 + lane < g.n) {
-              for (int r = 0; r < rows; ++r) {
-                const float value = block[r * 32 + (lane ^ r)];
-                const long long at = (row - lane + r) * g.ldc + col0 + lane;
-                if (g.out_kind == LC0B200_OUT_F32) reinterpret_cast<float*>(g.out)[at] = value;
-                else reinterpret_cast<bf16*>(g.out)[at] = __float2bfloat16_rn(value);
-              }
-            }
-            __syncwarp();
-          }
-        }
-      }
-      if (p.tma_store && n0 < g.n) {
-        ptx::fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-#pragma unroll
-          for (int i = 0; i < T::kGroups; ++i) {
-            if (n0 + 64 * i < g.n) {
-              ptx::tma_store_2d(&map_out, staging + i * kGroupBytes, n0 + 64 * i, static_cast<int>(row));
-            }
-          }
-          ptx::bulk_commit();
-        }
-      }
+      walk.next(num_groups, step_m, step_n, n_tiles);
+      fresh = !(p.tma_store && n0 < g.n && walk.tile < num_tiles);
+      if (kOverlap && !fresh) turn(Yes{}, Yes{});
+      else if (n0 < g.n) turn(Yes{}, No{});
     }
     if (p.tma_store && lane == 0) ptx::bulk_wait_read<0>();  // staging must outlive the last store's read
     __syncwarp();

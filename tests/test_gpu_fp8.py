@@ -395,6 +395,22 @@ def test_gemm_large(ops, m, n, k, dtype) -> None:
     assert torch.equal(again, out)
 
 
+# Several tiles per CTA pair whose finishing and first block run into one another: one block or two, ragged last columns.
+@pytest.mark.parametrize("activation", ["none", "mish", "swish"])
+@pytest.mark.parametrize("m, n, k", [(40000, 264, 128), (40000, 300, 100), (30011, 1000, 129), (70000, 40, 64), (20001, 1858, 256)])
+def test_gemm_many_tiles(ops, m, n, k, activation) -> None:
+    a, a_scale, w, w_scale = _operands(37, m, n, k)
+    up = -(-k // 16) * 16
+    a, w = _placed(a, up), _placed(w, up)
+    bias = torch.randn(n, generator=_gen(38)).to(BF16).cuda()
+    want, size = F8.gemm(a, a_scale, w, w_scale, bias, activation)
+    for dtype in (BF16, torch.float32):
+        out = _pitched(m, n, dtype, n + (-n % 8))
+        ops.gemm_fp8(out, a, a_scale, w, w_scale, bias=bias, activation=activation)
+        _close(out, want, size, k, activation)
+        _untouched(out)
+
+
 @pytest.mark.parametrize("m", [3, 64, 130, 600])
 def test_gemm_nan_stays_in_its_row_and_column(ops, m) -> None:
     n, k = 260, 640
