@@ -1,6 +1,7 @@
 // bf16 to e4m3 with one f32 scale per block (the rule is in fp8.cuh): 1 x 128 blocks along a row for activations,
 // 128 x 128 tiles for weights.  HBM-bound: three bytes an element move (two in, one out) and the values stay in
-// registers between the maximum and the rounding.
+// registers between the maximum and the rounding.  Aligned: 262144 x 1536 in 180 us (6.8 TB/s), 8190 x 8200 as tiles in 34
+// (6.0); any alignment: 65536 x 1001 in 50 us (4.0 TB/s).
 #include <cuda_runtime.h>
 
 #include "common.cuh"
@@ -107,12 +108,11 @@ quantize_fp8_odd_rows_kernel(uint8_t* __restrict__ q_out, float* __restrict__ sc
 // The maximum over a CTA's threads of magnitude bits.  `words` (one per warp) is used for every other tile only, so that the
 // next tile's writes cannot overtake this tile's reads.
 __device__ __forceinline__ uint32_t cta_max(uint32_t m, uint32_t* words) {
+  const int lane = threadIdx.x & 31;
   m = __reduce_max_sync(0xFFFFFFFFu, m);
-  if ((threadIdx.x & 31) == 0) words[threadIdx.x >> 5] = m;
+  if (lane == 0) words[threadIdx.x >> 5] = m;
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) m = max(m, words[w]);
-  return m;
+  return __reduce_max_sync(0xFFFFFFFFu, lane < kThreads / 32 ? words[lane] : 0u);
 }
 
 // One CTA per 128 x 128 tile, whole aligned words: each half-warp holds eight rows of the tile.
@@ -149,48 +149,63 @@ quantize_fp8_tiles_kernel(uint8_t* __restrict__ q_out, float* __restrict__ scale
 }
 
 // ... and for rows of any alignment and width: a warp holds every eighth row of the tile, channel lane + 32 i to a lane.
-__global__ void __launch_bounds__(kThreads)
+// Bound by the number of memory instructions (a channel each).  Four CTAs an SM, one's loads overlap another's stores:
+// 174775 x 846 in 105 us, 592 with one (175 registers a thread), 125 with three of 512 threads.  FULL: the tile lies
+// inside the matrix, nothing is checked per channel (215 us with the checks).
+constexpr int kOddCtas = 4;
+
+template <bool FULL>
+__device__ __forceinline__ void quantize_odd_tile(uint8_t* q, float* scale_out, const uint16_t* x, uint32_t* words, long long rows,
+                                                  int width, long long ld_in, long long ld_out) {
+  constexpr int kWarps = kThreads / 32, kRowsPerWarp = kFp8Block / kWarps;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint16_t* src = x + warp * ld_in + lane;
+  uint32_t raw[kRowsPerWarp][2];  // bf16 bits, two channels to a word
+  uint32_t m = 0u;
+#pragma unroll
+  for (int r = 0; r < kRowsPerWarp; ++r, src += kWarps * ld_in) {
+    uint32_t v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = FULL || (warp + kWarps * r < rows && lane + 32 * i < width) ? __ldg(src + 32 * i) : 0u;
+    raw[r][0] = v[0] | (v[1] << 16);
+    raw[r][1] = v[2] | (v[3] << 16);
+  }
+#pragma unroll
+  for (int r = 0; r < kRowsPerWarp; ++r) m = __vmaxu2(m, __vmaxu2(raw[r][0] & 0x7FFF7FFFu, raw[r][1] & 0x7FFF7FFFu));
+  float scale, inverse;
+  fp8_block_scale(cta_max(magnitude_of_packed(m), words), scale, inverse);
+  if (threadIdx.x == 0) *scale_out = scale;
+  uint8_t* dst = q + warp * ld_out + lane;
+#pragma unroll
+  for (int r = 0; r < kRowsPerWarp; ++r, dst += kWarps * ld_out) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float2 v = unpack_bf16x2(raw[r][i]);
+      const uint16_t codes = fp8_pack2(v.x * inverse, v.y * inverse);
+      if (FULL || (warp + kWarps * r < rows && lane + 64 * i < width)) dst[64 * i] = static_cast<uint8_t>(codes);
+      if (FULL || (warp + kWarps * r < rows && lane + 64 * i + 32 < width)) dst[64 * i + 32] = static_cast<uint8_t>(codes >> 8);
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kThreads, kOddCtas)
 quantize_fp8_odd_tiles_kernel(uint8_t* __restrict__ q_out, float* __restrict__ scale_out, const bf16* __restrict__ x, long long rows,
                               int width, long long ld_in, long long ld_out, long long ld_scale) {
   grid_dependency_release();
   grid_dependency_wait();
   __shared__ uint32_t warp_max[2][kThreads / 32];
-  constexpr int kWarps = kThreads / 32, kRowsPerWarp = kFp8Block / kWarps;
-  const int c0 = blockIdx.x * kFp8Block + (threadIdx.x & 31);
+  const int c0 = blockIdx.x * kFp8Block;
   const long long row_tiles = ceil_div_ll(rows, kFp8Block);
   int parity = 0;
   for (long long tile = blockIdx.y; tile < row_tiles; tile += gridDim.y, parity ^= 1) {
-    const long long row0 = tile * kFp8Block + (threadIdx.x >> 5);
-    uint32_t raw[kRowsPerWarp][2];  // bf16 bits, two channels to a word
-    uint32_t m = 0u;
-#pragma unroll
-    for (int r = 0; r < kRowsPerWarp; ++r) {
-      const long long row = row0 + kWarps * r;
-      const uint16_t* src = reinterpret_cast<const uint16_t*>(x) + row * ld_in + c0;
-      uint32_t v[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = row < rows && c0 + 32 * i < width ? __ldg(src + 32 * i) : 0u;
-      raw[r][0] = v[0] | (v[1] << 16);
-      raw[r][1] = v[2] | (v[3] << 16);
-    }
-#pragma unroll
-    for (int r = 0; r < kRowsPerWarp; ++r) m = __vmaxu2(m, __vmaxu2(raw[r][0] & 0x7FFF7FFFu, raw[r][1] & 0x7FFF7FFFu));
-    float scale, inverse;
-    fp8_block_scale(cta_max(magnitude_of_packed(m), warp_max[parity]), scale, inverse);
-    if (threadIdx.x == 0) scale_out[tile * ld_scale + blockIdx.x] = scale;
-#pragma unroll
-    for (int r = 0; r < kRowsPerWarp; ++r) {
-      const long long row = row0 + kWarps * r;
-      if (row < rows) {
-        uint8_t* dst = q_out + row * ld_out + c0;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float2 v = unpack_bf16x2(raw[r][i]);
-          const uint16_t codes = fp8_pack2(v.x * inverse, v.y * inverse);
-          if (c0 + 64 * i < width) dst[64 * i] = static_cast<uint8_t>(codes);
-          if (c0 + 64 * i + 32 < width) dst[64 * i + 32] = static_cast<uint8_t>(codes >> 8);
-        }
-      }
+    const long long row0 = tile * kFp8Block;
+    uint8_t* q = q_out + row0 * ld_out + c0;
+    float* scale = scale_out + tile * ld_scale + blockIdx.x;
+    const uint16_t* src = reinterpret_cast<const uint16_t*>(x) + row0 * ld_in + c0;
+    if (row0 + kFp8Block <= rows && c0 + kFp8Block <= width) {
+      quantize_odd_tile<true>(q, scale, src, warp_max[parity], kFp8Block, kFp8Block, ld_in, ld_out);
+    } else {
+      quantize_odd_tile<false>(q, scale, src, warp_max[parity], rows - row0, width - c0, ld_in, ld_out);
     }
   }
 }
