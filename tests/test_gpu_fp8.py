@@ -148,6 +148,17 @@ def test_quantize_long_and_wide(ops, rows, width) -> None:
         assert torch.equal(scale, want_scale)
 
 
+@pytest.mark.parametrize("rows, width", [(9000000, 7), (50000, 333)])
+def test_quantize_long_odd_tiles(ops, rows, width) -> None:
+    """More row tiles than a grid has in y: a CTA takes several, whole ones and the last short one."""
+    x = torch.randn((rows, width), device="cuda", generator=torch.Generator("cuda").manual_seed(4)).to(BF16)
+    want, want_scale = F8.quantize(x, 128)
+    out, scale = torch.empty((rows, width), dtype=FP8, device="cuda"), torch.empty_like(want_scale)
+    ops.quantize_fp8(out, scale, x, block_rows=128)
+    assert torch.equal(out.double(), want)
+    assert torch.equal(scale, want_scale)
+
+
 # ------------------------------------------------------------------ RMS norm
 
 def _check_norm(x, skip, gamma, epsilon, out, residual, q, scale) -> None:
