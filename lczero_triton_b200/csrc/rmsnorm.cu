@@ -249,23 +249,29 @@ __device__ __forceinline__ void store_run(const RmsParams& p, long long row, int
   }
 }
 
-template <int CHANNELS, bool SKIP, bool QUANT>
+// MANY: blockDim.y narrow rows a CTA.  With a CTA for every row the kernel is bound by how fast CTAs start (100000 rows of 61:
+// 104 us, 52 so); for rows of more than two warps one row is the faster (20000 x 1001: 43 us, 47 with two).
+template <int CHANNELS, bool SKIP, bool QUANT, bool MANY>
 __global__ void __launch_bounds__(1024) rms_norm_odd_kernel(const RmsParams p) {
   grid_dependency_release();
   grid_dependency_wait();
   __shared__ float warp_part[32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long row = blockIdx.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const long long row = MANY ? blockIdx.x * static_cast<long long>(blockDim.y) + threadIdx.y : blockIdx.x;
+  const bool here = !MANY || row < p.rows;
   const int c0 = 32 * CHANNELS * warp + lane;
   const bool full = 32 * CHANNELS * (warp + 1) <= p.width;
   float v[CHANNELS];
   bf16 gamma[CHANNELS];
-  float sum = warp_sum(full ? load_run<CHANNELS, SKIP, true>(p, row, c0, v, gamma) : load_run<CHANNELS, SKIP, false>(p, row, c0, v, gamma));
-  if (blockDim.x > 32) {
-    if (lane == 0) warp_part[warp] = sum;
+  float sum = 0.0f;
+  if (here) sum = warp_sum(full ? load_run<CHANNELS, SKIP, true>(p, row, c0, v, gamma) : load_run<CHANNELS, SKIP, false>(p, row, c0, v, gamma));
+  if (warps > 1) {
+    float* part = MANY ? warp_part + threadIdx.y * warps : warp_part;
+    if (lane == 0) part[warp] = sum;
     __syncthreads();
-    sum = warp_sum(lane < static_cast<int>(blockDim.x >> 5) ? warp_part[lane] : 0.0f);
+    sum = warp_sum(lane < warps ? part[lane] : 0.0f);
   }
+  if (!here) return;
   const float rstd = 1.0f / sqrtf(sum / static_cast<float>(p.width) + p.epsilon);
   if (full) store_run<CHANNELS, SKIP, QUANT, true>(p, row, c0, v, gamma, rstd);
   else store_run<CHANNELS, SKIP, QUANT, false>(p, row, c0, v, gamma, rstd);
@@ -341,14 +347,28 @@ void launch_words(const RmsParams& p, cudaStream_t st) {
   else launch_dependent(rms_norm_kernel<GROUPS, THREADS, false, false>, grid, block, 0, st, p);
 }
 
+template <int CHANNELS, bool MANY>
+void launch_odd(const RmsParams& p, dim3 grid, dim3 block, cudaStream_t st) {
+  const bool skip = p.skip != nullptr, quant = p.q != nullptr;
+  if (skip && quant) launch_dependent(rms_norm_odd_kernel<CHANNELS, true, true, MANY>, grid, block, 0, st, p);
+  else if (skip) launch_dependent(rms_norm_odd_kernel<CHANNELS, true, false, MANY>, grid, block, 0, st, p);
+  else if (quant) launch_dependent(rms_norm_odd_kernel<CHANNELS, false, true, MANY>, grid, block, 0, st, p);
+  else launch_dependent(rms_norm_odd_kernel<CHANNELS, false, false, MANY>, grid, block, 0, st, p);
+}
+
 template <int CHANNELS>
 void launch_odd(const RmsParams& p, cudaStream_t st) {
   const dim3 grid(static_cast<unsigned>(p.rows)), block(static_cast<unsigned>(32 * ceil_div_ll(p.width, 32 * CHANNELS)));
-  const bool skip = p.skip != nullptr, quant = p.q != nullptr;
-  if (skip && quant) launch_dependent(rms_norm_odd_kernel<CHANNELS, true, true>, grid, block, 0, st, p);
-  else if (skip) launch_dependent(rms_norm_odd_kernel<CHANNELS, true, false>, grid, block, 0, st, p);
-  else if (quant) launch_dependent(rms_norm_odd_kernel<CHANNELS, false, true>, grid, block, 0, st, p);
-  else launch_dependent(rms_norm_odd_kernel<CHANNELS, false, false>, grid, block, 0, st, p);
+  launch_odd<CHANNELS, false>(p, grid, block, st);
+}
+
+// Rows of one or two warps, up to four warps a CTA as long as there are eight CTAs for every SM.
+void launch_odd_narrow(const RmsParams& p, cudaStream_t st) {
+  const unsigned warps = p.width <= 256 ? 1 : 2;
+  unsigned rows_each = 1;
+  while (2 * rows_each * warps <= 4 && p.rows / (2 * rows_each) >= 8LL * sm_count()) rows_each *= 2;
+  const dim3 grid(static_cast<unsigned>(ceil_div_ll(p.rows, rows_each)));
+  launch_odd<8, true>(p, grid, dim3(32 * warps, rows_each), st);
 }
 
 // 16-byte accesses to every row of a bf16 operand that is there.
@@ -397,6 +417,10 @@ int rms_norm(void* out, void* residual, void* q_out, float* q_scale, const void*
     } else {
       launch_words<8, 256>(p, st);
     }
+    return launch_status();
+  }
+  if (width <= 512) {
+    launch_odd_narrow(p, st);
     return launch_status();
   }
   if (width <= 8192) {

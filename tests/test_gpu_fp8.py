@@ -200,6 +200,22 @@ def test_rms_norm(ops, rows, width, parts) -> None:
             _untouched(t)
 
 
+@pytest.mark.parametrize("rows, width", [(2367, 61), (2369, 300), (4739, 255), (9471, 257), (9473, 512), (5001, 7)])
+def test_rms_norm_many_narrow_rows(ops, rows, width) -> None:
+    """Several rows to a CTA, the last one not full, in and out of place."""
+    x, skip = _rows(17, rows, width), _rows(18, rows, width)
+    gamma = torch.randn(width + 1, generator=_gen(19)).to(BF16).cuda()[1:]
+    x_in, skip_in = x.clone(), skip.clone()
+    out, q = _pitched(rows, width, BF16, width + 3, 1), _pitched(rows, width, FP8, width + 1)
+    scale = _pitched(-(-width // 128), rows, torch.float32)
+    ops.rms_norm(out, x, gamma, skip=skip, q_out=q, q_scale=scale)
+    _check_norm(x, skip, gamma, 1e-6, out, None, q, scale)
+    for t in (out, q, scale):
+        _untouched(t)
+    ops.rms_norm(x, x, gamma, skip=skip, residual_out=skip)
+    _check_norm(x_in, skip_in, gamma, 1e-6, x, skip, None, None)
+
+
 @pytest.mark.parametrize("width", [96, 256, 1023, 2048, 3000, 17000])
 @pytest.mark.parametrize("offset, extra", [(0, 16), (8, 8), (1, 0), (2, 3)])
 def test_rms_norm_pitches(ops, width, offset, extra) -> None:
