@@ -1101,6 +1101,7 @@ int launch_few(const GemmFp8& g, cudaStream_t stream, const bf16* a_bf16 = nullp
 
 }  // namespace
 
+// (The Python wrapper counts launches by the same rule.)
 bool linear_fp8_few_supported(const GemmFp8& g, const bf16* a, long long lda) {
   return g.m <= 16 && (g.k % 8) == 0 && aligned16(a) && (lda % 8 == 0 || g.m == 1) && aligned16(g.w) && (g.ldw % 16 == 0 || g.n == 1);
 }

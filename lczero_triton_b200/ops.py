@@ -393,9 +393,13 @@ def linear_fp8(out: torch.Tensor, a: torch.Tensor, w: torch.Tensor, w_scale: tor
     _scratch(scratch_scale, "scratch_scale", torch.float32, m * -(-k // FP8_BLOCK), device)
     if m == 0:
         return out
-    check(_lib.load().lc0b200_linear_fp8(_p(out), _p(a), _p(w), _p(w_scale), _p(bias), _p(scratch_q), _p(scratch_scale),
+    rows, weight = a.data_ptr(), w.data_ptr()
+    # The library's own rule for the form that quantises inside the product (lc0b200_linear_fp8).
+    one = (m <= 16 and k % 8 == 0 and rows % 16 == 0 and (lda % 8 == 0 or m == 1) and weight % 16 == 0
+           and (ldw % 16 == 0 or n == 1))
+    check(_lib.load().lc0b200_linear_fp8(_p(out), rows, weight, _p(w_scale), _p(bias), _p(scratch_q), _p(scratch_scale),
                                          m, n, k, lda, ldw, ld_w_scale, ldc, kind,
-                                         ACTIVATIONS[activation], _raw_stream(device)), "linear_fp8", launches=1 if m <= 16 else 2)
+                                         ACTIVATIONS[activation], _raw_stream(device)), "linear_fp8", launches=1 if one else 2)
     return out
 
 
