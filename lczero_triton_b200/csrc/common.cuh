@@ -8,6 +8,7 @@
 #include <atomic>
 
 #include "../../include/lc0b200.h"
+#include "per_device.h"
 
 namespace lc0b200 {
 
@@ -18,7 +19,6 @@ using bf16 = __nv_bfloat16;
 //   status: device address of four status words on THAT device.  Word 0: first device-side failure
 //   code (0 = none); word 1: detail (role / barrier index); word 2: CTA; word 3: parity waited for.
 //   Written by kernels whose bounded waits ran out; read and cleared by lc0b200_device_status().
-constexpr int kMaxDevices = 64;
 struct DeviceInfo {
   int index;
   int sm_count;

@@ -1014,15 +1014,19 @@ int launch(const GemmFp8& g, cudaStream_t stream) {
   auto kernel = gemm_fp8_kernel<BN, CTAS, ACT>;
   static PerDeviceOnce smem_opt_in;  // per instantiation
   if (allow_dynamic_smem(smem_opt_in, kernel, T::kSmemBytes) != LC0B200_OK) return LC0B200_ERR_CUDA;
-  if (T::kSplitRegs) {
-    // A register split that asks for more than the launch has would wait for ever.
-    static const int launch_regs = [](auto k) {
+  if constexpr (T::kSplitRegs) {
+    // A register split that asks for more than the launch has would wait for ever; the 128-wide tile needs none.
+    static PerDeviceNumber launch_regs;  // per instantiation
+    const DeviceInfo* device = device_info();
+    if (device == nullptr) return LC0B200_ERR_CUDA;
+    const int regs = ask_once(launch_regs, device->index, [&] {
       cudaFuncAttributes attributes;
-      if (cudaFuncGetAttributes(&attributes, k) == cudaSuccess) return attributes.numRegs;
+      if (cudaFuncGetAttributes(&attributes, kernel) == cudaSuccess) return attributes.numRegs;
       (void)cudaGetLastError();
       return 0;
-    }(kernel);
-    if (launch_regs < T::kLaunchRegs) return LC0B200_ERR_UNSUPPORTED;
+    });
+    if (regs == 0) return LC0B200_ERR_CUDA;
+    if (regs < T::kLaunchRegs) return launch<128, 1, ACT>(g, stream);
   }
   const long long tiles = ceil_div_ll(g.m, kBM * CTAS) * ceil_div_ll(g.n, BN);
   const long long max_groups = sm_count() / CTAS;
