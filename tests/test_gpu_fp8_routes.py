@@ -68,3 +68,20 @@ def test_linear_counts_its_launches(ops, m, k, extra, offset, w_extra) -> None:
     before = _lib.launch_count()
     launched = _kernels(lambda: ops.linear_fp8(out, x, w, w_scale, None, *scratch))
     assert _lib.launch_count() - before == len(launched), launched
+
+
+# ------------------------------------------------------------------ the CUDA-core product
+
+@pytest.mark.parametrize("n", [64 * 65535, 64 * 65535 + 1, 64 * 70000 + 130])
+def test_cuda_core_product_of_many_columns(ops, n) -> None:
+    """More tiles of 64 columns than a grid has in y."""
+    m, k = 3, 5
+    a = torch.randint(-8, 9, (m, k), generator=_gen(72)).float().to(FP8).cuda()
+    w = torch.randint(-8, 9, (n, k), generator=torch.Generator("cuda").manual_seed(73), device="cuda").float().to(FP8)
+    a_scale = torch.tensor([[1.0, 0.5, 2.0]], device="cuda")
+    w_scale = torch.exp2(torch.randint(-3, 4, (-(-n // 128), 1), generator=torch.Generator("cuda").manual_seed(74), device="cuda").float())
+    out = _pitched(m, n, torch.float32)
+    assert _kernels(lambda: ops.gemm_fp8(out, a, a_scale, w, w_scale)) == [f"gemm_fp8_simt_kernel<{str(n > 64 * 65535).lower()}>"]
+    # Small whole numbers times powers of two: every step is exact.
+    want = (a.float() @ w.float().t()) * a_scale.t() * w_scale.repeat_interleave(128)[:n]
+    assert torch.equal(out, want)
