@@ -287,15 +287,18 @@ LC0B200_API int lc0b200_quantize_fp8(void* out_e4m3, float* scale_f32, const voi
  * y = v / sqrt(mean(v^2) + epsilon) * gamma, fp32; out = bf16(y) and / or q_out, q_scale = block rule on y (each pair may
  * be NULL, not both).  Every output is rounded once from its fp32 value.  out and residual_out may be in or skip
  * themselves (same pointer and pitch).  A pitch belongs to its pointer and is ignored where that is NULL.
- * v * gamma is formed first and the sum of squares is fp32: y is wanted where both are finite fp32 numbers.  A row of
- * finite values whose sum of squares overflows (values above 1e19 / sqrt(width) or so) gives zeros. */
+ * v * gamma is formed first and the sum of squares is fp32.  y is as exact as fp32 makes it where both are finite, every
+ * v * gamma is zero or at least 2^-126, and mean(v^2) + epsilon is at least 2^-126 (with an epsilon of 1e-6 or so it always
+ * is; with 0, a row has to reach a root mean square of 2^-63).  Below these limits bits are lost; a row whose sum of squares
+ * vanishes divides by zero if epsilon is 0 (infinities, NaN for zeros).  A row of finite values whose sum of squares
+ * overflows (values above 1e19 / sqrt(width) or so) gives zeros. */
 LC0B200_API int lc0b200_rms_norm(void* out_bf16, void* residual_out_bf16, void* q_out_e4m3, float* q_scale_f32,
                                  const void* in_bf16, const void* skip_bf16, const void* gamma_bf16, long long row_count,
                                  int width, float epsilon, long long ld_in, long long ld_skip, long long ld_out,
                                  long long ld_residual, long long ld_q, long long ld_scale, void* stream);
 /* out[m,n] = act(bias[n] + sum over 128-blocks b of k: a_scale[b,m] * w_scale[n / 128, b] * sum_{k in b} a[m,k] * w[n,k]),
  * codes [m,k] and [n,k] row-major, fp32 sums, bias bf16 or NULL, out bf16 or f32 (out_kind).  The two scales of a block are
- * multiplied in fp32 first, so their product has to be a finite fp32 number.  A NaN stays in its row of a and its
+ * multiplied in fp32 first, so their product has to be a finite fp32 number (below 2^-126 it loses bits).  A NaN stays in its row of a and its
  * column of w.  Bases and pitches of a and w that are multiples of 16 bytes run on the tensor cores, others on the CUDA
  * cores (correct, slow).  The order of summation depends on shape, alignment and device alone: the same call gives the
  * same bits. */

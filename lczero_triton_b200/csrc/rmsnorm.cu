@@ -3,8 +3,9 @@
 //   y = v / sqrt(mean(v^2) + eps) * gamma
 //   out = bf16(y), and / or e4m3 codes with a scale per 1 x 128 block of the f32 y (fp8.cuh)
 // Every result is rounded once, from the f32 value: the norm reads v and not the rounded residual, the codes come from
-// y and not from the bf16 row, so that no result depends on which of the others are asked for.  y = (v * gamma) * rstd: the
-// product of two bf16 values is exact, and as rstd is a factor of the whole row, the codes come from v * gamma alone.
+// y and not from the bf16 row, so that no result depends on which of the others are asked for.  y = (v * gamma) * rstd:
+// without a skip v * gamma is a product of two bf16 values and exact (with one, v is an f32 sum and the product rounds), and as
+// rstd is a factor of the whole row, the codes come from v * gamma alone.
 // HBM-bound: a row is read once and kept in registers (rows of more than 16384 channels are read twice).  262144 x 1024 with
 // skip, residual, bf16 and codes: 360 us, 6.8 TB/s.  One row of 4096: 1.9 us, latency.  Rows of any alignment are bound by
 // the number of memory instructions: 5003 x 1111 with skip and residual in 11.3 us, its bytes take 6.8.

@@ -14,7 +14,7 @@ import torch
 from torch.autograd import DeviceType
 from torch.profiler import ProfilerActivity, profile
 
-from test_gpu_fp8 import BF16, FP8, _gen, _operands, _pitched, _placed, _rows, _scratch
+from test_gpu_fp8 import BF16, FP8, _check_norm, _gen, _operands, _pitched, _placed, _rows, _scratch
 
 pytestmark = pytest.mark.gpu
 
@@ -85,3 +85,35 @@ def test_cuda_core_product_of_many_columns(ops, n) -> None:
     # Small whole numbers times powers of two: every step is exact.
     want = (a.float() @ w.float().t()) * a_scale.t() * w_scale.repeat_interleave(128)[:n]
     assert torch.equal(out, want)
+
+
+# ------------------------------------------------------------------ RMS norm
+
+@pytest.mark.parametrize("rows", [3, 200])
+@pytest.mark.parametrize("width", [64, 256, 1024, 1111, 4096, 9001, 17000])
+@pytest.mark.parametrize("of_x, of_gamma, epsilon", [(-62, 0, 0.0), (-62, -40, 0.0), (-62, 60, 0.0), (-75, 0, 2.0 ** -126)])
+def test_rms_norm_at_its_lower_limit(ops, rows, width, of_x, of_gamma, epsilon) -> None:
+    """mean(v^2) + epsilon from 2^-126 on.  Squares below fp32's normal range are off by 2^-150 at the most, so the mean is:
+    one rounding relative to 2^-126, half of one in the result.  The tolerance has it to spare (16 additions are counted for
+    the trees, which have 13 at the most)."""
+    x, skip = _rows(75, rows, width) * 2.0 ** of_x, _rows(76, rows, width) * 2.0 ** of_x
+    gamma = ((1 + 0.2 * torch.randn(width, generator=_gen(77))) * 2.0 ** of_gamma).to(BF16).cuda()
+    v = x.double() + skip.double()
+    assert bool((v.square().mean(dim=1) + epsilon >= 2.0 ** -126).all())
+    least = (v * gamma.double()).abs()
+    assert bool(((least == 0) | (least >= 2.0 ** -126)).all())
+    out, q = torch.empty((rows, width), dtype=BF16, device="cuda"), torch.empty((rows, width), dtype=FP8, device="cuda")
+    scale = torch.empty((-(-width // 128), rows), device="cuda")
+    ops.rms_norm(out, x, gamma, epsilon=epsilon, skip=skip, q_out=q, q_scale=scale)
+    _check_norm(x, skip, gamma, epsilon, out, None, q, scale)
+
+
+@pytest.mark.parametrize("width", [64, 1111, 2048, 20000])
+def test_rms_norm_whose_squares_vanish(ops, width) -> None:
+    """Below the limit, as documented: infinities without an epsilon, and with one the formula's tiny values."""
+    x, gamma = torch.full((2, width), 2.0 ** -76, dtype=BF16, device="cuda"), torch.ones(width, dtype=BF16, device="cuda")
+    out = torch.empty_like(x)
+    ops.rms_norm(out, x, gamma, epsilon=0.0)
+    assert bool((out == float("inf")).all())
+    ops.rms_norm(out, x, gamma, epsilon=1e-6)
+    _check_norm(x, None, gamma, 1e-6, out, None, None, None)
