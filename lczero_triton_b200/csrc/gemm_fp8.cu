@@ -117,14 +117,33 @@ __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_add
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
-// After a wait that ran out: the loads under way still write into this CTA's memory.  Waits for the last one of every stage,
-// a millisecond at the most; `stage` and `phase` are where the next load would have gone.
+// After a wait that ran out, each for a millisecond at the most:
+constexpr uint64_t kDrainLimitNs = 1000000;
+// The loads under way still write into this CTA's memory.  Waits for the last one of every stage; `stage` and `phase` are where
+// the next load would have gone.  The loads of a pair complete on the leader's barriers, and its peer may have issued one
+// that the leader did not get to: both rest for the whole millisecond.
+template <int CTAS>
 __device__ __forceinline__ void drain_loads(uint32_t bar_full, int stages, int stage, uint32_t phase) {
   const uint64_t start = ptx::globaltimer_ns();
-  for (int s = 0; s < stages; ++s) {
+  for (int s = 0; CTAS == 1 && s < stages; ++s) {
     const uint32_t parity = s < stage ? phase : phase ^ 1u;
-    while (!ptx::mbar_try_wait(bar_full + 8 * s, parity) && ptx::globaltimer_ns() - start < 1000000u) {
+    while (!ptx::mbar_try_wait(bar_full + 8 * s, parity) && ptx::globaltimer_ns() - start < kDrainLimitNs) {
     }
+  }
+  while (CTAS == 2 && ptx::globaltimer_ns() - start < kDrainLimitNs) {
+  }
+}
+// The MMAs under way still read shared memory and write tensor memory (a pair's in both CTAs).  Called by the lane that issued
+// them: its commit arrives at `bar_done` once they have ended.
+template <int CTAS>
+__device__ __forceinline__ void drain_mmas(uint32_t bar_done) {
+  if (CTAS == 2) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(ptx::map_to_cta(bar_done, 0u)) : "memory");
+  } else {
+    ptx::tc_commit<1>(bar_done);
+  }
+  const uint64_t start = ptx::globaltimer_ns();
+  while (!ptx::mbar_try_wait(bar_done, 0u) && ptx::globaltimer_ns() - start < kDrainLimitNs) {
   }
 }
 
@@ -297,8 +316,9 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
   const uint32_t bar_scale_empty = bar_part_empty + 8 * kPartials;      // [kPartials]
   const uint32_t tmem_slot = bar_scale_empty + 8 * kPartials;
   const uint32_t scale_base = bar_base + T::kBarrierBytes;              // [kPartials][kScaleCols][kBM] f32
+  const uint32_t bar_done = tmem_slot + 8;  // for drain_mmas alone
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem_raw + (tmem_slot + 4 - smem_base));
-  static_assert(16 * kStages + 24 * kPartials + 8 <= T::kBarrierBytes, "barrier area too small");
+  static_assert(16 * kStages + 24 * kPartials + 16 <= T::kBarrierBytes, "barrier area too small");
   grid_dependency_release();
   if ((smem_base & 1023u) != 0u) {  // never seen; refuse loudly rather than mis-swizzle
     if (threadIdx.x == 0 && atomicCAS(&p.status[0], 0u, kDeviceSmemMisaligned) == 0u) p.status[1] = smem_base;
@@ -327,6 +347,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       ptx::mbar_init(bar_part_empty + 8 * a, T::kEpilogueWarps * CTAS);
       ptx::mbar_init(bar_scale_empty + 8 * a, T::kEpilogueWarps);
     }
+    ptx::mbar_init(bar_done, 1);
     ptx::mbar_init_fence();
     ptx::prefetch_tensormap(&map_a);
     ptx::prefetch_tensormap(&map_w);
@@ -377,11 +398,14 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
           }
         }
       }
-      if (!ok && rank == 0) drain_loads(bar_full, kStages, stage, phase);
+      if (!ok) drain_loads<CTAS>(bar_full, kStages, stage, phase);
       __syncwarp();
     } else if (warp == 1) {
       // ------------------------------------------------------------ MMAs (leader CTA only): one partial per k block
-      if (rank == 0) {
+      // One lane runs the whole loop: it may give up by itself.  (With the warp in step around an elected lane every wait has to
+      // be followed by a vote: 2048 x 1024 x 4096 on 128-wide tiles in 15.6 us, 14.3 without votes, 13.1 so; on pair tiles
+      // the three are within half a per cent.)
+      if (rank == 0 && ptx::elect_one()) {
         int stage = 0, part = 0;
         uint32_t phase = 0, part_phase = 0;
         bool ok = true;
@@ -397,14 +421,12 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             ok = ok && ptx::mbar_wait(bar_part_empty + 8 * part, part_phase ^ 1u, abort_flag, p.status, 0x1200u + part);
             if (!ok) break;
             ptx::tc_fence_after_sync();
-            if (ptx::elect_one()) {
 #pragma unroll
-              for (int j = 0; j < kFp8Block / kMmaK; ++j) {
-                mma_e4m3<CTAS>(tmem_base + part * BN, a_desc + j * (kMmaK >> 4), b_desc + j * (kMmaK >> 4), idesc, j > 0 ? 1u : 0u);
-              }
-              ptx::tc_commit<CTAS>(bar_part_full + 8 * part);
-              ptx::tc_commit<CTAS>(bar_empty + 8 * stage);
+            for (int j = 0; j < kFp8Block / kMmaK; ++j) {
+              mma_e4m3<CTAS>(tmem_base + part * BN, a_desc + j * (kMmaK >> 4), b_desc + j * (kMmaK >> 4), idesc, j > 0 ? 1u : 0u);
             }
+            ptx::tc_commit<CTAS>(bar_part_full + 8 * part);
+            ptx::tc_commit<CTAS>(bar_empty + 8 * stage);
             if (++stage == kStages) {
               stage = 0;
               phase ^= 1u;
@@ -415,6 +437,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             }
           }
         }
+        if (!ok) drain_mmas<CTAS>(bar_done);
       }
       __syncwarp();
     } else {
@@ -482,10 +505,10 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     static_assert(kChunks % 2 == 0, "a block's first columns go to the first buffer");
     uint64_t acc[T::kCols / 2];
     float scale = 0.0f;
-    // Waits for the next partial and fetches its scale.
+    // Waits for the next partial and fetches its scale.  A wait that ran out changes nothing yet: lanes must not part before
+    // the tensor-memory loads that follow (of whatever is there), and the vote on `ok` comes after them, where it costs nothing.
     auto begin_block = [&](float& block_scale) {
       ok = ptx::mbar_wait(bar_part_full + 8 * part, part_phase, abort_flag, p.status, 0x1400u + part);
-      if (!ok) return;
       ptx::tc_fence_after_sync();
       asm volatile("ld.shared.f32 %0, [%1];" : "=f"(block_scale) : "r"(my_scale + part * T::kScaleBytes) : "memory");
     };
@@ -557,8 +580,11 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     // 262144 x 1536 x 1024 with mish: 611 us with one after the other, 580 so.
     auto turn = [&](auto finish, auto take) {
       constexpr bool kFinish = decltype(finish)::value, kTake = decltype(take)::value;
-      if (kTake) begin_block(scale);
-      if (kTake && !ok) return;
+      if (kTake) {
+        begin_block(scale);
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        if (!ok) return;
+      }
       const int this_part = kTake ? take_part() : 0;
       uint64_t scale2 = 0ull;
       uint32_t w[32];
@@ -621,6 +647,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       if (k_blocks > kTaken) {
         begin_block(scale);
         ptx::tmem_ld_32x32(tmem_row + part * BN, v[0]);
+        ok = __all_sync(0xFFFFFFFFu, ok);
       }
       for (int kb = kTaken; kb < k_blocks && ok; ++kb) {
         const uint64_t scale2 = both_f32x2(scale);
@@ -635,6 +662,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             if (kb + 1 < k_blocks) {
               begin_block(scale);
               ptx::tmem_ld_32x32(tmem_row + part * BN, v[0]);
+              ok = __all_sync(0xFFFFFFFFu, ok);
             }
           }
 #pragma unroll
@@ -730,8 +758,9 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
   const uint32_t bar_part_empty = bar_part_full + 8 * kPartials;    // [kPartials]
   const uint32_t tmem_slot = bar_part_empty + 8 * kPartials;
   const uint32_t scale_base = bar_base + T::kBarrierBytes;          // [kPartials][NT] f32
+  const uint32_t bar_done = tmem_slot + 8;  // for drain_mmas alone
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem_raw + (tmem_slot + 4 - smem_base));
-  static_assert(16 * kStages + 16 * kPartials + 8 <= T::kBarrierBytes, "barrier area too small");
+  static_assert(16 * kStages + 16 * kPartials + 16 <= T::kBarrierBytes, "barrier area too small");
   grid_dependency_release();
 
   const int warp = threadIdx.x >> 5;
@@ -762,6 +791,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
       ptx::mbar_init(bar_part_full + 8 * a, 2);   // the MMAs' completion and a scale warp
       ptx::mbar_init(bar_part_empty + 8 * a, T::kEpilogueWarps);
     }
+    ptx::mbar_init(bar_done, 1);
     ptx::mbar_init_fence();
     ptx::prefetch_tensormap(&map_w);
     if (!BF16_A) ptx::prefetch_tensormap(&map_a);
@@ -798,7 +828,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         phase ^= 1u;
       }
     }
-    if (!ok) drain_loads(bar_full, kStages, stage, phase);
+    if (!ok) drain_loads<1>(bar_full, kStages, stage, phase);
     __syncwarp();
   } else if (warp == 1) {
     constexpr uint32_t idesc = ptx::instr_desc(1u, 0u, 0u, kBM, NT);
@@ -828,6 +858,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         part_phase ^= 1u;
       }
     }
+    if (!ok && ptx::elect_one()) drain_mmas<1>(bar_done);
     __syncwarp();
   } else if (warp < 4) {
     // Scales: two warps take the k blocks in turn; lane j holds the products of tokens j and j + 32.
