@@ -374,7 +374,7 @@ def test_gemm_activations(ops, activation, m, n, k) -> None:
         _close(out, want, size, k, activation)
 
 
-# Few rows, then both tile shapes, each with the CUDA-core form beside it (an odd pitch).
+# Few rows, the CUDA-core form (an odd pitch) and pair tiles; every other kernel is in test_gpu_fp8_routes.py.
 @pytest.mark.parametrize("activation", ["mish", "relu", "swish"])
 @pytest.mark.parametrize("m, pitch", [(3, 128), (70, 128), (70, 129), (4000, 128), (6000, 128)])
 def test_gemm_activation_range(ops, activation, m, pitch) -> None:
