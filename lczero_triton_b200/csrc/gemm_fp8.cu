@@ -16,8 +16,6 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
-#include <type_traits>
-
 #include "common.cuh"
 #include "fp8.cuh"
 #include "gemm_fp8.h"
@@ -530,13 +528,12 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       }
       return taken;
     };
-    constexpr bool kOverlap = CTAS == 2;  // tiles of one CTA are for problems of about one tile each
-    constexpr int kTaken = kOverlap ? 1 : 0;
+    constexpr int kTaken = CTAS == 2 ? 1 : 0;  // blocks of a tile in front of the loop; tiles of one CTA are about one to a CTA
     long long row = 0;  // of the tile whose sums are being formed or finished
     int n0 = 0;
-    // Stores the 32 columns from col0 on, chunk c of the tile; `tma`: into the staging buffers of a tensor map's store.
-    auto store_chunk = [&](int c, int col0, uint64_t (&y)[16], bool tma) {
-      if (tma) {
+    // Stores the 32 columns from col0 on, chunk c of the tile, or leaves them in the staging buffers of a tensor map's store.
+    auto store_chunk = [&](int c, int col0, uint64_t (&y)[16]) {
+      if (p.tma_store) {
         // Row `lane` of the group's 32 x 128-byte buffer, 16-byte chunk i at i ^ (lane & 7): the 128-byte swizzle.
         const uint32_t row_addr = staging + (c >> 1) * kGroupBytes + lane * kRowBytes;
 #pragma unroll
@@ -574,47 +571,43 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       __syncwarp();
     };
 
-    // After a tile's last block.  FINISH: bias, activation and store, 32 columns at a time.  TAKE: the next tile's first block
-    // into registers that are free; with both, what finishing frees, so that its columns are on their way while the stores
-    // are issued and the MMAs get the partial back earlier (only for results a tensor map stores, which issue quickly).
-    // 262144 x 1536 x 1024 with mish: 611 us with one after the other, 580 so.
-    auto turn = [&](auto finish, auto take) {
-      constexpr bool kFinish = decltype(finish)::value, kTake = decltype(take)::value;
-      if (kTake) {
-        begin_block(scale);
-        ok = __all_sync(0xFFFFFFFFu, ok);
-        if (!ok) return;
-      }
-      const int this_part = kTake ? take_part() : 0;
-      uint64_t scale2 = 0ull;
+    // A tile's first block sets the sums, where a tile ends behind another's: no additions to zeros.  (Started from zeros as
+    // tiles of one CTA are, 262144 x 1536 x 1024 takes 535 us instead of 515.)
+    auto take_first = [&]() {
+      begin_block(scale);
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      if (!ok) return;
+      const int this_part = take_part();
+      const uint64_t scale2 = both_f32x2(scale);
       uint32_t w[32];
-      if (kFinish && (kTake || p.tma_store)) {
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        ptx::tmem_ld_32x32(tmem_row + this_part * BN + 32 * c, w);
+        tmem_wait(w);
+        if (c + 1 == kChunks) end_block(this_part);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) acc[c * 16 + j] = mul_f32x2(pack_f32x2(w[2 * j], w[2 * j + 1]), scale2);
+      }
+    };
+    // After a tile's last block: bias, activation and store, 32 columns at a time.  (With the next tile's first block taken into
+    // the registers that this frees, 32 columns at a time as well, 262144 x 1536 x 1024 gained half a per cent without an
+    // activation and lost 3 with mish, and results that no tensor map stores lost 4 to 10 to the larger kernel.)
+    auto finish = [&]() {
+      if (p.tma_store) {
         if (lane == 0) ptx::bulk_wait_read<0>();  // the staging buffers are free once the last tile's stores have read them
         __syncwarp();
       }
 #pragma unroll
       for (int c = 0; c < kChunks; ++c) {
         const int col0 = n0 + 32 * c;
+        if (col0 >= g.n) break;
         uint64_t y[16];
-        if (kFinish && (kTake || col0 < g.n)) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) y[j] = acc[c * 16 + j];
-          finish32<ACT>(y, g, col0);
-          if (kTake) ptx::tmem_ld_32x32(tmem_row + this_part * BN + 32 * c, w);
-          store_chunk(c, col0, y, kTake || p.tma_store);
-        } else if (kTake) {
-          ptx::tmem_ld_32x32(tmem_row + this_part * BN + 32 * c, w);
-        }
-        if (kTake) {
-          tmem_wait(w);
-          if (c == 0) scale2 = both_f32x2(scale);
-          if (c + 1 == kChunks) end_block(this_part);
-#pragma unroll
-          for (int j = 0; j < 16; ++j) acc[c * 16 + j] = mul_f32x2(pack_f32x2(w[2 * j], w[2 * j + 1]), scale2);
-        }
+        for (int j = 0; j < 16; ++j) y[j] = acc[c * 16 + j];
+        finish32<ACT>(y, g, col0);
+        store_chunk(c, col0, y);
       }
-      // After the partial is back with the MMAs: this takes 650 cycles.
-      if (kFinish && (kTake || p.tma_store)) {
+      if (p.tma_store) {
         ptx::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
@@ -627,19 +620,16 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       }
     };
 
-    using Yes = std::true_type;
-    using No = std::false_type;
     TileWalk walk(group, n_tiles);
-    bool fresh = true;  // no block of the tile has been taken
     while (walk.tile < num_tiles && ok) {
-      if (kOverlap && fresh) turn(No{}, Yes{});
+      if (kTaken > 0) take_first();
       if (!ok) break;
       row = walk.m * kTileM + rank * kBM + quarter * 32 + lane;
       n0 = walk.n * BN + half * T::kCols;
       // 32 columns at a time: while they are added, the next 32 are on their way, across the k blocks too (a partial is
       // handed back, and the next one's first columns asked for, before the last additions).  Columns past the matrix
       // edge hold anything and are not stored.
-      if (!kOverlap) {
+      if (kTaken == 0) {
 #pragma unroll
         for (int i = 0; i < T::kCols / 2; ++i) acc[i] = 0ull;
       }
@@ -674,9 +664,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         break;
       }
       walk.next(num_groups, step_m, step_n, n_tiles);
-      fresh = !(p.tma_store && n0 < g.n && walk.tile < num_tiles);
-      if (kOverlap && !fresh) turn(Yes{}, Yes{});
-      else if (n0 < g.n) turn(Yes{}, No{});
+      if (n0 < g.n) finish();
     }
     if (p.tma_store && lane == 0) ptx::bulk_wait_read<0>();  // staging must outlive the last store's read
     __syncwarp();
