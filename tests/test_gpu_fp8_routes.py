@@ -7,7 +7,10 @@ Tolerances are those of test_gpu_fp8.py, which counts the roundings.
 
 from __future__ import annotations
 
+import pathlib
 import re
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -267,6 +270,48 @@ def test_products_at_once_and_replayed(ops, route) -> None:
         states[0]["x"].copy_(inputs[which])
         graph.replay()
         assert torch.equal(states[0]["out"], want[which]) and torch.equal(states[0]["layer"], want[which])
+
+
+FIRST_CALLS = """
+import torch
+from lczero_triton_b200 import ops
+bf16, fp8 = torch.bfloat16, torch.float8_e4m3fn
+calls, results = [], []
+for m, n, k in ((4, 256, 512), (61, 7496, 256), (1000, 1352, 256), (3000, 840, 256), (40, 100, 257)):
+    x = torch.randn((m, k), device="cuda").to(bf16)
+    w, gamma = torch.randn((n, k), device="cuda").to(bf16), torch.ones(k, dtype=bf16, device="cuda")
+    q, s = torch.empty((m, k), dtype=fp8, device="cuda"), torch.empty((-(-k // 128), m), device="cuda")
+    wq, ws = torch.empty((n, k), dtype=fp8, device="cuda"), torch.empty((-(-n // 128), -(-k // 128)), device="cuda")
+    outs = [torch.empty((m, n), dtype=bf16, device="cuda") for _ in range(2)]
+    scratch = torch.empty(m * -(-k // 16) * 16, dtype=fp8, device="cuda"), torch.empty(m * -(-k // 128), device="cuda")
+    def call(x=x, w=w, gamma=gamma, q=q, s=s, wq=wq, ws=ws, outs=outs, scratch=scratch):
+        ops.quantize_fp8(wq, ws, w, block_rows=128)
+        ops.rms_norm(None, x, gamma, q_out=q, q_scale=s)
+        ops.gemm_fp8(outs[0], q, s, wq, ws, activation="mish")
+        ops.linear_fp8(outs[1], x, wq, ws, None, *scratch)
+    calls.append(call)
+    results += outs
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    for call in calls:
+        call()
+graph.replay()
+kept = [r.clone() for r in results]
+for r in results:
+    r.zero_()
+for call in calls:
+    call()
+assert all(torch.equal(r, k) for r, k in zip(results, kept))
+print("captured first")
+"""
+
+
+def test_first_calls_of_a_process_may_be_captured(ops) -> None:
+    """Nothing that a first call sets up (attributes, addresses, tensor maps) is forbidden while a stream is captured."""
+    root = pathlib.Path(__file__).resolve().parents[1]
+    done = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "captured first" in done.stdout, done.stderr[-2000:]
 
 
 # ------------------------------------------------------------------ launches that the binding counts
