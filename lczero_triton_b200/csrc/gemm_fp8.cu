@@ -8,11 +8,13 @@
 // gemm_fp8_kernel (many rows): persistent, tiles of 128 x BN per CTA, or 256 x 256 per CTA pair (cta_group::2; each CTA
 // loads its own rows of A and its own half of W with plain TMA loads, none is multicast).  Warp 0 loads (one elected
 // lane), warp 1 issues the MMAs, warps 2 and 3 bring the scales, warps 4 and up are the epilogue: two per TMEM lane quarter,
-// each with half of the columns.  Bound by the way of a partial through the epilogue and back (740 cycles a block against
-// 512 of MMA, with the two partials that fit), then by what ends a tile, and back to back by the power limit.
-// 32768 x 1024 x 4096: 125 us, 2200 TFLOP/s; 65536 x 1024 x 1024: 75 us; 32768 x 1536 x 1024 with mish: 86 us.
-// gemm_fp8_few_kernel (few rows): further down.  Bound by the weight's bytes, or by latency: 1 x 4096 x 4096 in 6.4 us,
-// 1 x 16384 x 16384 in 52 (5.2 TB/s).
+// each with half of the columns.  Bound by the way of a partial through the epilogue and back (710 cycles a block against
+// 512 of MMA, with the two partials that fit), then by what ends a tile (3500 cycles, 8400 with mish), and back to back by
+// the power limit.  Ten launches after a rest / launches back to back for seconds, us: 32768 x 1024 x 4096: 125 (2200 TFLOP/s) /
+// 146; 65536 x 1024 x 1024: 74 / 87; 32768 x 1536 x 1024 with mish: 88 / 89; 32768 x 1024 x 1024: 42 / 45, to f32 70 / 71.
+// Other figures of single kernels here are of the first kind.
+// gemm_fp8_few_kernel (few rows): further down.  Bound by the weight's bytes, or by latency: 1 x 4096 x 4096 in 6.3 us,
+// 1 x 16384 x 16384 in 48 (5.6 TB/s).
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -545,7 +547,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
       }
       // f32 results and rows a tensor map cannot address: turn the 32 x 32 block in shared memory (element c of
       // row r at c ^ r, no bank conflicts either way) and write whole rows, 32 neighbouring elements a store, eight rows in
-      // flight (20000 x 1858 x 1024 with mish: 106 us, 130 row by row).
+      // flight (20000 x 1858 x 1024 with mish, back to back: 93 us, a quarter more row by row).
       float* block = reinterpret_cast<float*>(smem_raw + (staging - smem_base));
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
@@ -572,7 +574,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     };
 
     // A tile's first block sets the sums, where a tile ends behind another's: no additions to zeros.  (Started from zeros as
-    // tiles of one CTA are, 262144 x 1536 x 1024 takes 535 us instead of 515.)
+    // tiles of one CTA are, 262144 x 1536 x 1024 takes 535 us back to back instead of 515.)
     auto take_first = [&]() {
       begin_block(scale);
       ok = __all_sync(0xFFFFFFFFu, ok);

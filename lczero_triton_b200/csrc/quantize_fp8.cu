@@ -1,7 +1,7 @@
 // bf16 to e4m3 with one f32 scale per block (the rule is in fp8.cuh): 1 x 128 blocks along a row for activations,
 // 128 x 128 tiles for weights.  HBM-bound: three bytes an element move (two in, one out) and the values stay in
-// registers between the maximum and the rounding.  Aligned: 262144 x 1536 in 180 us (6.8 TB/s), 8190 x 8200 as tiles in 34
-// (6.0); any alignment: 65536 x 1001 in 50 us (4.0 TB/s).
+// registers between the maximum and the rounding.  Aligned: 262144 x 1536 in 182 us (6.7 TB/s), 8190 x 8200 as tiles in 37
+// (5.4); any alignment: 65536 x 1001 in 52 us (3.8 TB/s).
 #include <cuda_runtime.h>
 
 #include "common.cuh"
@@ -150,7 +150,7 @@ quantize_fp8_tiles_kernel(uint8_t* __restrict__ q_out, float* __restrict__ scale
 
 // ... and for rows of any alignment and width: a warp holds every eighth row of the tile, channel lane + 32 i to a lane.
 // Bound by the number of memory instructions (a channel each).  Four CTAs an SM, one's loads overlap another's stores:
-// 174775 x 846 in 105 us, 592 with one (175 registers a thread), 125 with three of 512 threads.  FULL: the tile lies
+// 174775 x 846 in 108 us, 592 with one (175 registers a thread), 125 with three of 512 threads.  FULL: the tile lies
 // inside the matrix, nothing is checked per channel (215 us with the checks).
 constexpr int kOddCtas = 4;
 

@@ -6,7 +6,8 @@
 // y and not from the bf16 row, so that no result depends on which of the others are asked for.  y = (v * gamma) * rstd:
 // without a skip v * gamma is a product of two bf16 values and exact (with one, v is an f32 sum and the product rounds), and as
 // rstd is a factor of the whole row, the codes come from v * gamma alone.
-// HBM-bound: a row is read once and kept in registers (rows of more than 16384 channels are read twice).  262144 x 1024 with
+// HBM-bound: a row is read once and kept in registers (rows of more than 16384 channels are read twice, a channel an access
+// whatever their alignment: 2048 x 20480 with skip and residual in 147 us, 2.3 TB/s, where 16384 channels take 47).  262144 x 1024 with
 // skip, residual, bf16 and codes: 360 us, 6.8 TB/s.  One row of 4096: 1.9 us, latency.  Rows of any alignment are bound by
 // the number of memory instructions: 5003 x 1111 with skip and residual in 11.3 us, its bytes take 6.8.
 #include <cuda_runtime.h>
@@ -175,7 +176,8 @@ __global__ void __launch_bounds__(THREADS == 32 ? 32 * kWarpsPerBlock : 256) rms
 // Rows of any alignment and width: a warp takes a run of 32 CHANNELS channels, channel run + lane + 32 i to a lane, so that
 // a warp's access is one run of memory and four channels of a lane make a 128-block; as many warps a row as it has runs.
 // Eight channels a lane keep many rows in flight: with a whole row of 1111 to a warp (48 channels a lane, 137 registers) 5003
-// rows took 27 us.  (16-byte or 4-byte words shifted into place move fewer requests and execute three times the instructions.)
+// rows took 27 us.  (16-byte or 4-byte words shifted into place move fewer requests and execute three times the instructions: 26 and
+// 37 us, with a whole row to a warp; with eight channels a lane they were not tried.)
 // FULL: the run lies inside the row, nothing is checked per channel.
 template <int CHANNELS, bool SKIP, bool FULL>
 __device__ __forceinline__ float load_run(const RmsParams& p, long long row, int c0, float (&v)[CHANNELS], bf16 (&gamma)[CHANNELS]) {

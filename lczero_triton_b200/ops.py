@@ -359,7 +359,7 @@ def gemm_fp8(out: torch.Tensor, a: torch.Tensor, a_scale: torch.Tensor, w: torch
     """``out[m,n] = act(a @ w.T + bias)`` of e4m3 codes ``a [m,k]``, ``w [n,k]`` with a scale per block
     (``include/lc0b200.h``: lc0b200_gemm_fp8): ``a_scale [ceil(k/128), m]``, ``w_scale [ceil(n/128), ceil(k/128)]``.
     ``out`` is bf16 or f32.  Keep row pitches and bases of ``a`` and ``w`` at multiples of 16 bytes: others run on
-    the CUDA cores."""
+    the CUDA cores, 20 to 60 times slower."""
     device = _device_of(a, "a")
     m, k = a.shape
     lda = _matrix(a, torch.float8_e4m3fn, "a", m, k, device)
@@ -380,7 +380,8 @@ def gemm_fp8(out: torch.Tensor, a: torch.Tensor, a_scale: torch.Tensor, w: torch
 def linear_fp8(out: torch.Tensor, a: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: torch.Tensor | None,
                scratch_q: torch.Tensor, scratch_scale: torch.Tensor, *, activation: str = "none") -> torch.Tensor:
     """bf16 activations -> e4m3 codes and scales (into caller scratch) -> ``gemm_fp8``.  ``scratch_q`` is any contiguous
-    tensor of at least ``m * (k rounded up to 16)`` bytes, ``scratch_scale`` of at least ``m * ceil(k/128)`` floats."""
+    e4m3 tensor of at least ``m * (k rounded up to 16)`` elements, ``scratch_scale`` of at least ``m * ceil(k/128)`` floats,
+    both 16-byte aligned."""
     device = _device_of(a, "a")
     m, k = a.shape
     lda = _matrix(a, torch.bfloat16, "a", m, k, device)
