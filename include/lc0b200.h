@@ -298,10 +298,10 @@ LC0B200_API int lc0b200_rms_norm(void* out_bf16, void* residual_out_bf16, void* 
                                  long long ld_residual, long long ld_q, long long ld_scale, void* stream);
 /* out[m,n] = act(bias[n] + sum over 128-blocks b of k: a_scale[b,m] * w_scale[n / 128, b] * sum_{k in b} a[m,k] * w[n,k]),
  * codes [m,k] and [n,k] row-major, fp32 sums, bias bf16 or NULL, out bf16 or f32 (out_kind).  The two scales of a block are
- * multiplied in fp32 first, so their product has to be a finite fp32 number (below 2^-126 it loses bits).  A NaN stays in its row of a and its
- * column of w.  Bases and pitches of a and w that are multiples of 16 bytes run on the tensor cores, others on the CUDA
- * cores (correct, 20 to 60 times slower: 8192 x 1024 x 1001 in 0.8 ms instead of 16 us).  The order of summation depends on shape, alignment and device alone: the same call gives the
- * same bits. */
+ * multiplied in fp32 first, so their product has to be a finite fp32 number (below 2^-126 it loses bits).  A NaN stays in its
+ * row of a and its column of w.  Bases and pitches of a and w that are multiples of 16 bytes run on the tensor cores, others
+ * on the CUDA cores (correct, 20 to 60 times slower: 8192 x 1024 x 1001 in 0.8 ms instead of 16 us).  The order of summation
+ * depends on shape, alignment and device alone: the same call gives the same bits. */
 LC0B200_API int lc0b200_gemm_fp8(void* out, const void* a_e4m3, const float* a_scale, const void* w_nk_e4m3,
                                  const float* w_scale, const void* bias_bf16, long long m, int n, int k, long long lda,
                                  long long ld_a_scale, long long ldw, long long ld_w_scale, long long ldc, int out_kind,
